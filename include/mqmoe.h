@@ -361,6 +361,34 @@ int mq_w4a16_tc_swiglu(const void* xp, const float* xs,
                        int64_t H, int64_t group_size, void* h_shuffled, int32_t* d_status, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * W8A8 (no counterpart in the reference): int8 weights with an fp32 scale for each output channel, int8 rows with an
+ * fp32 scale for each row, int32 sums.
+ *
+ * mq_quantize_rows_int8: row_scale = max|x| / 127 rounded to fp32, q = the whole number nearest to x / row_scale (the
+ *   exact quotient, halves to even), in -127..127.  A row of zeros: scale 0, q 0.  A row that holds an infinity or a NaN:
+ *   scale NaN, q 0 (what is computed from it is NaN).  x: rows of K elements, row_stride elements apart (any alignment);
+ *   q [rows,K] dense, scale [rows].  Limits: rows < 2^31.
+ * mq_w8a8_grouped_gemm: out[r,n] = round(float(sum_k x[r,k] * w[e][n,k]) * x_scale[r] * w_scale[e][n]) for the rows r of
+ *   group e; x int8 [S,Kd], qweight int8 [weight_period, N, Kd], w_scale fp32 [weight_period, N], offsets int32 [E+1],
+ *   out [S,N] of out_dtype, rows outside the groups untouched; weight_period as in mq_grouped_gemm.
+ * mq_w8a8_linear: the same with one group of M rows and no offsets.
+ * mq_w8a8_grouped_swiglu: h[r,:] = round(silu(g) * u) of the unrounded fp32 products with the gate and the up rows of
+ *   w_gate_up [weight_period, 2*I, H] (gate rows first), w_scale [weight_period, 2*I].  perm != NULL: row r of the sorted
+ *   order is row perm[r] / top_k of x [T,H], gathered inside the kernel (S entries); NULL: x holds the S sorted rows, T = S.
+ * Limits: Kd <= 131071 (the sums are exact in 32 bits), rows and groups < 2^30, N < 2^29. */
+int mq_quantize_rows_int8(const void* x, int dtype, int64_t rows, int64_t K, int64_t row_stride, int8_t* q, float* scale,
+                          void* stream);
+int mq_w8a8_grouped_gemm(const int8_t* x, const float* x_scale, const int8_t* qweight, const float* w_scale,
+                         const int32_t* offsets, int64_t S, int64_t E, int64_t weight_period, int64_t N, int64_t Kd,
+                         int out_dtype, void* out, int32_t* d_status, void* stream);
+int mq_w8a8_linear(const int8_t* x, const float* x_scale, const int8_t* qweight, const float* w_scale, int64_t M, int64_t N,
+                   int64_t Kd, int out_dtype, void* out, int32_t* d_status, void* stream);
+int mq_w8a8_grouped_swiglu(const int8_t* x, const float* x_scale, const int32_t* perm, int64_t T, int64_t top_k,
+                           const int8_t* w_gate_up, const float* w_scale, const int32_t* offsets, int64_t S, int64_t E,
+                           int64_t weight_period, int64_t I, int64_t H, int out_dtype, void* h, int32_t* d_status,
+                           void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * The whole block in one call: what Qwen3MoEBlock.forward (mini_qwen/model/layers/moe.py:49-68) computes on one
  * GPU, as the chain of the calls above with every intermediate in one caller workspace.  norm_weight != NULL puts
  * the decoder layer's RMSNorm in front, residual != NULL its add behind (mini_qwen/model/qwen3_moe.py:63-66);

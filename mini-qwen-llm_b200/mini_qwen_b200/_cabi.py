@@ -53,6 +53,10 @@ PROTOTYPES = {
     "mq_w4a16_tc_prep": (c_int, [_P, _P, _L, _L, _L, _I, _P, _P, _P]),
     "mq_w4a16_tc_gemm": (c_int, [_P, _P, _P, _P, _P, _P, _L, _L, _L, _L, _L, _L, _P, _P, _P]),
     "mq_w4a16_tc_swiglu": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _L, _L, _L, _L, _L, _L, _P, _P, _P]),
+    "mq_quantize_rows_int8": (c_int, [_P, _I, _L, _L, _L, _P, _P, _P]),
+    "mq_w8a8_grouped_gemm": (c_int, [_P, _P, _P, _P, _P, _L, _L, _L, _L, _L, _I, _P, _P, _P]),
+    "mq_w8a8_linear": (c_int, [_P, _P, _P, _P, _L, _L, _L, _I, _P, _P, _P]),
+    "mq_w8a8_grouped_swiglu": (c_int, [_P, _P, _P, _L, _L, _P, _P, _P, _L, _L, _L, _L, _L, _I, _P, _P, _P]),
     "mq_moe_forward_workspace_bytes": (c_size_t, [_P, _L]),
     "mq_moe_forward": (c_int, [_P, _P, _P, c_float, _P, _L, _P, c_size_t, _P, c_size_t, _P, _P, _P, _P]),
     "mq_ep_share_counts": (c_int, [_P, _L, _L, _L, _P, _P]),
@@ -134,6 +138,33 @@ def require_cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise ValueError("these kernels run on CUDA tensors only; there is no CPU path")
+
+
+def one_device(*tensors: torch.Tensor | None) -> torch.device:
+    """The device that all of a call's tensors lie on."""
+    require_cuda(*tensors)
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"the tensors of a call lie on one device; got {device} and {t.device}")
+    return device
+
+
+class current_device:
+    """Launches inside go to ``device``, whichever is the current one (a no-op where it already is)."""
+
+    def __init__(self, device: torch.device):
+        self._index, self._before = device.index, None
+
+    def __enter__(self):
+        now = torch.cuda.current_device()
+        if self._index is not None and self._index != now:
+            torch.cuda.set_device(self._index)
+            self._before = now
+
+    def __exit__(self, *exc):
+        if self._before is not None:
+            torch.cuda.set_device(self._before)
 
 
 def check(status: int, what: str) -> None:
