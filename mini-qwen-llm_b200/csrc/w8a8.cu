@@ -4,12 +4,16 @@
 // Follows the shapes of mini_qwen/kernels/moe_grouped_gemm.py:17-37 and mini_qwen/model/layers/moe.py:24-25; the
 // reference has no 8-bit path.  The int32 sums are exact (K <= 131071: 128 * 128 * K < 2^31).
 //
-// This file: the entry points, and the kernel for every shape and alignment (dot products of four bytes, tiles of 64 rows
-// by 64 columns through shared memory).
-#include "tc5.cuh"
+// This file: the entry points, and the kernel for what the tensor-core kernel (w8a8_pair.cu) leaves: any size and alignment
+// (dot products of four bytes, tiles of 64 rows by 64 columns through shared memory).
 #include "w8a8.cuh"
 
 namespace mq {
+
+// Tensor cores, CTA pairs (w8a8_pair.cu).
+bool w8a8_pair_covers(const W8Args& A, bool swiglu);
+int w8a8_pair(const W8Args& A, bool swiglu, int out_dtype, int32_t* d_status, cudaStream_t st);
+
 namespace {
 
 constexpr int G_M = 64, G_N = 64, G_K = 64;        // rows, columns and bytes of k of a tile
@@ -129,6 +133,7 @@ int w8a8_dispatch(W8Args A, bool swiglu, int out_dtype, int32_t* d_status, cudaS
   if (A.S == 0) return MQ_OK;
   if (A.T == 0 || !A.x || !A.x_scale || !A.w || !A.w_scale || !A.out) return MQ_ERR_INVALID_ARGUMENT;
   if (A.perm == nullptr && A.T < A.S) return MQ_ERR_INVALID_ARGUMENT;
+  if (w8a8_pair_covers(A, swiglu)) return w8a8_pair(A, swiglu, out_dtype, d_status, st);
   A.words = ((A.K | (int)(reinterpret_cast<uintptr_t>(A.x) & 3u) | (int)(reinterpret_cast<uintptr_t>(A.w) & 3u)) & 3) == 0;
   if (out_dtype == MQ_F32) return launch_generic<float>(A, swiglu, st);
   if (out_dtype == MQ_BF16) return launch_generic<__nv_bfloat16>(A, swiglu, st);

@@ -28,6 +28,10 @@ __device__ __forceinline__ size_t w8_source(const W8Args& A, int row) {
 __device__ __forceinline__ float w8_value(int sum, float row_scale, float channel_scale) {
   return __fmul_rn(__fmul_rn(__int2float_rn(sum), row_scale), channel_scale);
 }
-__device__ __forceinline__ float w8_swiglu(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) * u, with the exponential of -|g| so that nothing overflows and the quotient's denominator is in 1..2.
+__device__ __forceinline__ float w8_swiglu(float g, float u) {
+  const float p = expf(-fabsf(g));
+  return __fdividef(g < 0.0f ? p * g : g, 1.0f + p) * u;
+}
 
 }  // namespace mq
