@@ -397,13 +397,15 @@ int mq_w8a8_grouped_swiglu(const int8_t* x, const float* x_scale, const int32_t*
  * residual and out are [T, hidden] of L->dtype, as x is.
  *   dense layers (group_size 0, any dtype): gate[0] = w13 [E, 2*inter, hidden] (gate rows, then up rows),
  *     down[0] = w2 [E, hidden, inter];
- *   W4A16 layers (dtype MQ_BF16): gate / up / down = {qweight, scales, qzeros} of the stacks.
+ *   W4A16 layers (dtype MQ_BF16): gate / up / down = {qweight, scales, qzeros} of the stacks;
+ *   W8A8 layers (int8_experts != 0, group_size 0; dtype: that of x and out): gate = {w13 int8 [E, 2*inter, hidden],
+ *     scales fp32 [E, 2*inter]}, down = {w2 int8 [E, hidden, inter], scales fp32 [E, hidden]} (mq_moe_small only).
  * route_workspace: as mq_route_small's (zero-filled once by the caller, for 64 tokens, kept between calls that are
  * ordered with one another); read for T <= 64 only.  workspace: mq_moe_forward_workspace_bytes(layer, T) bytes,
  * overwritten.  h_launches (optional) receives the number of kernels launched. */
 typedef struct {
   int64_t hidden, inter, experts, top_k, group_size;
-  int32_t dtype, router_dtype, renormalize, reserved;
+  int32_t dtype, router_dtype, renormalize, int8_experts;
   const void* router;            /* [experts, hidden] */
   const float* router_bias;      /* [experts] or NULL */
   const void* gate[3];
@@ -415,6 +417,24 @@ int mq_moe_forward(const mq_moe_layer* h_layer, const void* x, const void* norm_
                    const void* residual, int64_t T, void* route_workspace, size_t route_workspace_bytes,
                    void* workspace, size_t workspace_bytes, void* out, int32_t* d_status,
                    int32_t* h_launches, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * The same layer for up to 16 tokens in two launches (what Qwen3MoEBlock.forward computes, layers/moe.py:49-68), with one
+ * rounding at the end instead of one after every operation:
+ *   out[t] = round(sum_k weight[t,k] * down[e](silu(gate[e](x[t])) * up[e](x[t])) + residual[t]),
+ * the top_k experts of a token being those with the largest logits (equal ones by ascending id).  W8A8 layers quantise x
+ * and h to int8 per token, as mq_quantize_rows_int8 does.  residual may be NULL; out may alias x or residual only where
+ * nothing else reads them (out == residual is allowed, out == x is not).
+ * mq_moe_small_covers: whether T tokens of the layer are covered: T <= 16, experts <= 1024, top_k <= 32; bf16 or fp16 experts
+ *   with hidden and inter multiples of 8; W4A16 with group sizes that are multiples of 128; W8A8 with multiples of 16 whose
+ *   T * top_k rows of h fit the shared memory (about 190 KB).
+ * workspace: mq_moe_small_workspace_bytes(layer, T) bytes, 16-byte aligned, overwritten; calls that may overlap on the GPU
+ *   need one each.  x and the weights are 16-byte aligned.  The second launch is cooperative: one CTA on every SM, which
+ *   meet once; d_status (optional) receives MQ_DEV_WAIT_EXPIRED if that wait ran out, and out is then not written. */
+int mq_moe_small_covers(const mq_moe_layer* h_layer, int64_t T);
+size_t mq_moe_small_workspace_bytes(const mq_moe_layer* h_layer, int64_t T);
+int mq_moe_small(const mq_moe_layer* h_layer, const void* x, const void* residual, int64_t T, void* workspace,
+                 size_t workspace_bytes, void* out, int32_t* d_status, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Expert parallelism over peer memory (no counterpart in the reference, which is single-GPU).

@@ -96,7 +96,7 @@ size_t carve(const mq_moe_layer& L, int64_t T, const BlockPlan& p, bool norm, ui
 
 bool layer_ok(const mq_moe_layer* L) {
   return L != nullptr && L->hidden > 0 && L->inter > 0 && L->experts > 0 && L->top_k > 0 && L->group_size >= 0 &&
-         valid_dtype(L->dtype) && valid_dtype(L->router_dtype) && (L->group_size == 0 || L->dtype == MQ_BF16);
+         valid_dtype(L->dtype) && valid_dtype(L->router_dtype) && !L->int8_experts && (L->group_size == 0 || L->dtype == MQ_BF16);
 }
 
 }  // namespace

@@ -59,6 +59,9 @@ PROTOTYPES = {
     "mq_w8a8_grouped_swiglu": (c_int, [_P, _P, _P, _L, _L, _P, _P, _P, _L, _L, _L, _L, _L, _I, _P, _P, _P]),
     "mq_moe_forward_workspace_bytes": (c_size_t, [_P, _L]),
     "mq_moe_forward": (c_int, [_P, _P, _P, c_float, _P, _L, _P, c_size_t, _P, c_size_t, _P, _P, _P, _P]),
+    "mq_moe_small_covers": (c_int, [_P, _L]),
+    "mq_moe_small_workspace_bytes": (c_size_t, [_P, _L]),
+    "mq_moe_small": (c_int, [_P, _P, _P, _L, _P, c_size_t, _P, _P, _P]),
     "mq_ep_share_counts": (c_int, [_P, _L, _L, _L, _P, _P]),
     "mq_ep_barrier": (c_int, [_P, _P, _L, _L, _L, _P, _P]),
     "mq_ep_plan": (c_int, [_P, _L, _L, _L, _P, _P, _P]),
@@ -75,7 +78,7 @@ PROTOTYPES = {
 class MoELayer(ctypes.Structure):
     """``mq_moe_layer``: what a whole-block call needs to know about a layer."""
     _fields_ = ([(n, c_int64) for n in ("hidden", "inter", "experts", "top_k", "group_size")]
-                + [(n, ctypes.c_int32) for n in ("dtype", "router_dtype", "renormalize", "reserved")]
+                + [(n, ctypes.c_int32) for n in ("dtype", "router_dtype", "renormalize", "int8_experts")]
                 + [("router", c_void_p), ("router_bias", c_void_p)]
                 + [(n, c_void_p * 3) for n in ("gate", "up", "down")])
 
