@@ -426,11 +426,10 @@ int mq_moe_forward(const mq_moe_layer* h_layer, const void* x, const void* norm_
  * and h to int8 per token, as mq_quantize_rows_int8 does.  residual may be NULL; out may alias x or residual only where
  * nothing else reads them (out == residual is allowed, out == x is not).
  * mq_moe_small_covers: whether T tokens of the layer are covered: T <= 16, experts <= 1024, top_k <= 32; bf16 or fp16 experts
- *   with hidden and inter multiples of 8; W4A16 with group sizes that are multiples of 128; W8A8 with multiples of 16 whose
- *   T * top_k rows of h fit the shared memory (about 190 KB).
+ *   with hidden and inter multiples of 8; W4A16 with group sizes that are multiples of 128; W8A8 with multiples of 16.
  * workspace: mq_moe_small_workspace_bytes(layer, T) bytes, 16-byte aligned, overwritten; calls that may overlap on the GPU
  *   need one each.  x and the weights are 16-byte aligned.  The second launch is cooperative: one CTA on every SM, which
- *   meet once; d_status (optional) receives MQ_DEV_WAIT_EXPIRED if that wait ran out, and out is then not written. */
+ *   wait for one another; d_status (optional) receives MQ_DEV_WAIT_EXPIRED if a wait ran out, and out is then invalid. */
 int mq_moe_small_covers(const mq_moe_layer* h_layer, int64_t T);
 size_t mq_moe_small_workspace_bytes(const mq_moe_layer* h_layer, int64_t T);
 int mq_moe_small(const mq_moe_layer* h_layer, const void* x, const void* residual, int64_t T, void* workspace,

@@ -17,12 +17,14 @@
 //     rows of all experts hit are dealt out evenly, to the row, so that no CTA has more than its share of bytes; one barrier
 //     over the grid; then each CTA takes a few output columns of ALL experts hit, so the sum over experts stays inside the
 //     CTA: no atomics, no second pass, the same bits every time;
-//   * a warp reads 16-byte pieces of weight rows straight into registers, in an order of k in which they are the fragments
-//     of mma.sync (tokens are its 8 columns): the tensor cores cost nothing here, and eight tokens of an expert cost one pass
-//     over its weights.  The next pieces are in flight while one batch is multiplied; the first ones of the down projection
-//     are issued, and the rest of its weights asked into L2, before the barrier.
-// The wait at the barrier is bounded; when it runs out, MQ_DEV_WAIT_EXPIRED is set and nothing is written.
+//   * the weights come by tensor-map copies, issued by one warp, through a ring of 128 to 160 KB that runs on through the
+//     barrier, so that the first weights of the down projection arrive under it.  Sixteen warps multiply: a lane's 16-byte
+//     pieces are, in a suitable order of k, the fragments of mma.sync (tokens are its 8 columns), so the tensor cores cost
+//     nothing here, and all tokens of an expert cost one pass over its weights.  Three warps finish the tiles of h.
+//     (A warp copying for itself, through registers or a ring of its own, spent its time on addresses: 3.7 TB/s.)
+// Every wait is bounded; when one runs out, MQ_DEV_WAIT_EXPIRED is set and the output is invalid.
 #include "int8.cuh"
+#include "tc5.cuh"
 
 namespace mq {
 namespace {
@@ -30,9 +32,9 @@ namespace {
 using namespace int8;
 
 constexpr int MAX_T = 16, MAX_E = 1024, MAX_K = 32;
-constexpr int WARPS = 16, THREADS = WARPS * 32;
-constexpr int BATCH = 4;                           // steps of k a warp has in flight
-constexpr size_t SMEM_LIMIT = 229376;              // dynamic shared memory, beside the static 2 KB
+constexpr int WARPS = 16;                          // that multiply
+constexpr int FINISH = 3;                          // that finish the tiles of h; one more issues the copies
+constexpr int THREADS = (WARPS + FINISH + 1) * 32;
 constexpr uint32_t POLL_LIMIT = 1u << 22;          // looks at the barrier: about two seconds
 
 enum Format { F_BF16, F_F16, F_INT8, F_INT4 };
@@ -48,10 +50,12 @@ struct SmallArgs {
   const __nv_bfloat16* sc[3];
   const int32_t* qz[3];
   int T, H, I, E, K, group, renorm, dtype, router_dtype;
+  int tile, box_rows;                              // columns of h in a tile; rows of a down box, or word rows of an int4 gate box
   unsigned* counter;                               // workspace from here on
   uint32_t* amax;                                  // [T * K] largest |h| of a slot, as bits
   float* logits;                                   // [T, E]
   int8_t* xq;                                      // [T, H]
+  int8_t* hq;                                      // [T * K, I]
   float* xs;                                       // [T]
   void* h;                                         // bf16, int4: [T * K, 2, I] high and low parts; else fp32 [T * K, I]
   int32_t* d_status;
@@ -149,18 +153,6 @@ __global__ void __launch_bounds__(128) moe_small_router(const SmallArgs A, int r
 
 // ---- launch 2 -------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ uint4 ld_weights(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ld_weights2(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
-
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -252,62 +244,111 @@ __device__ __forceinline__ void select_experts(const float* logits, int E, int K
   }
 }
 
-// Tables in shared memory behind the partial sums.
+// Tables in shared memory behind the rings and the sums.
 struct Tables {
   uint32_t* mask;      // [E] tokens of the expert
   uint16_t* pos;       // [E] its place among the experts hit
-  uint16_t* hit;       // [hits]
-  uint16_t* before;    // [hits] slots of the experts in front of it
-  uint8_t* slot;       // [hits, MAX_T] which of the token's experts it is
-  float* weight;       // [hits, MAX_T] its weight in the token's sum
-  uint16_t* ids;       // [T, MAX_K]
-  float* w;            // [T, MAX_K]
+  uint16_t* hit;       // [hits] the expert
+  uint8_t* count;      // [hits] its tokens; they are columns 0, 1, ... of its products:
+  uint16_t* slot;      // [hits, MAX_T] token * MAX_K + which of its experts it is
+  uint16_t* ids;       // [T, MAX_K] the tokens' experts
+  float* w;            // [T, MAX_K] and their weights
   __host__ __device__ static size_t bytes(int T, int E, int K) {
     const size_t hits = (size_t)(E < T * K ? E : T * K);
-    return hits * MAX_T * 5 + hits * 4 + (size_t)E * 6 + (size_t)T * MAX_K * 6 + 64;
+    return hits * (MAX_T * 2 + 3) + (size_t)E * 6 + (size_t)T * MAX_K * 6 + 16;
   }
   __device__ Tables(uint8_t* p, int T, int E, int K) {
     const int hits = min(E, T * K);
-    weight = reinterpret_cast<float*>(p);
-    w = weight + hits * MAX_T;
+    w = reinterpret_cast<float*>(p);
     mask = reinterpret_cast<uint32_t*>(w + T * MAX_K);
-    ids = reinterpret_cast<uint16_t*>(mask + E);
+    slot = reinterpret_cast<uint16_t*>(mask + E);
+    ids = slot + hits * MAX_T;
     pos = ids + T * MAX_K;
     hit = pos + E;
-    before = hit + hits;
-    slot = reinterpret_cast<uint8_t*>(before + hits);
+    count = reinterpret_cast<uint8_t*>(hit + hits);
   }
 };
 
-// Weight bytes per k and elements of k in a step of 64 bytes (int4: 32 k, four words of a column).
-template <int F> struct Fmt { static constexpr int STEP = F == F_INT8 ? 64 : 32, SIZE = F == F_INT8 ? 1 : 2; };
-
-constexpr int PARTS = 64;                          // 16 x 8 partial sums that a meeting of the warps holds
-constexpr int PART_BUFFER = PARTS * 512;           // their bytes for eight tokens
-constexpr int SUM_BUFFER = WARPS * 512;            // the same of the output's sums
-__host__ __device__ constexpr size_t part_bytes(int octets) { return (size_t)2 * PART_BUFFER * octets; }
-// Shared memory in front of the tables: the partial sums, later the output's sums and (int8) the quantised h.
-__host__ __device__ inline size_t front_bytes(bool int8, int octets, int64_t slots, int64_t I) {
-  const size_t later = (size_t)2 * SUM_BUFFER * octets + (int8 ? (size_t)slots * (I + 16) : 0);
-  return later > part_bytes(octets) ? (later + 15) & ~(size_t)15 : part_bytes(octets);
+// A unit is what a warp multiplies at a time: 128 bytes of k of 16 weight rows (gate and up: 8 of either), or int4 words:
+// 128 k of 16 columns of gate and up, 256 k of 16 columns of down.  A stage of the ring holds a unit for each warp.
+template <int F> struct Fmt {
+  static constexpr bool W4 = F == F_INT4;
+  static constexpr int SIZE = F == F_INT8 ? 1 : 2;
+  static constexpr int UNIT_K = W4 ? 128 : 128 / SIZE, UNIT2_K = W4 ? 256 : 128 / SIZE;
+  static constexpr int MT = W4 ? 2 : 1;            // accumulator tiles: int4 gate and up apart, else 8 + 8 rows in one
+};
+constexpr int UNIT = 2048, STAGE = WARPS * UNIT;
+// Stages of the ring; the partial sums (two buffers) and the tables lie behind it.
+__host__ __device__ constexpr int ring_stages(int f, int octets) { return f == F_INT4 && octets == 2 ? 4 : 5; }
+__host__ __device__ constexpr size_t part_bytes(int f, int octets) { return (size_t)WARPS * 512 * (f == F_INT4 ? 2 : 1) * octets; }
+__host__ __device__ constexpr size_t front_bytes(int f, int octets) {
+  return (size_t)ring_stages(f, octets) * STAGE + 2 * part_bytes(f, octets);
 }
 
+// One barrier over the grid; `arrive` may come well before `wait`.  Thread 0 of each CTA, between barriers of the CTA.
+__device__ __forceinline__ void grid_arrive(unsigned* counter) {
+  __threadfence();
+  atomicAdd(counter, 1u);
+}
+__device__ __forceinline__ bool grid_wait(unsigned* counter, unsigned target) {
+  uint32_t seen = 0, looks = 0;
+  do {
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
+  } while (seen < target && ++looks < POLL_LIMIT);
+  __threadfence();
+  return seen >= target;
+}
+
+// The copies, from the weights' tensor maps.
+__device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+               ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+__device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+               ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+// A barrier of some of the CTA's warps.
+template <int ID, int N> __device__ __forceinline__ void warps_meet() { asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N * 32) : "memory"); }
+
+struct SmallMaps { CUtensorMap gate, up, down; };  // dense and int8: gate and up rows in one
+
 template <int F, int OCT, typename OutT>
-__global__ void __launch_bounds__(THREADS, 1) moe_small_layer(const SmallArgs A) {
+__global__ void __launch_bounds__(THREADS, 1) moe_small_layer(const SmallArgs A, const __grid_constant__ SmallMaps maps) {
+  using namespace tc5;
   using Acc = typename std::conditional<F == F_INT8, int, float>::type;
-  constexpr int STEP = Fmt<F>::STEP, SIZE = Fmt<F>::SIZE;
+  constexpr int SIZE = Fmt<F>::SIZE, UNIT_K = Fmt<F>::UNIT_K, UNIT2_K = Fmt<F>::UNIT2_K, MT = Fmt<F>::MT;
   constexpr bool W4 = F == F_INT4;
-  constexpr int TW = W4 ? 16 : 8;                  // columns of h in a tile
-  constexpr int MT = W4 ? 2 : 1;                   // accumulator tiles: int4 gate and up apart, else 8 + 8 rows in one
-  extern __shared__ uint8_t small_smem[];
-  uint8_t* part = small_smem;
-  const Tables tab(small_smem + front_bytes(F == F_INT8, OCT, A.T * A.K, A.I), A.T, A.E, A.K);
-  __shared__ int s_hits, s_ok;
-  __shared__ int4 s_tile[2][PARTS];                // expert's place, first column, columns
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
+  constexpr int STAGES = ring_stages(F, OCT);
+  constexpr int HP = F == F_INT8 ? 1 : 2;          // 16-byte pieces of h per step and lane in the down projection
+  extern __shared__ uint8_t small_smem_raw[];
+  uint8_t* const small_smem = small_smem_raw + ((1024u - (smem_addr(small_smem_raw) & 1023u)) & 1023u);   // the copies' swizzle
+  uint8_t* part = small_smem + STAGES * STAGE;
+  const Tables tab(small_smem + front_bytes(F, OCT), A.T, A.E, A.K);
+  __shared__ int s_hits, s_ok, s_abort;
+  __shared__ __align__(8) uint64_t s_bars[2 * STAGES + 4];
+  const uint32_t bars = smem_addr(s_bars), ring = smem_addr(small_smem);
+  auto full = [&](int i) { return bars + 8u * i; };
+  auto empty = [&](int i) { return bars + 8u * (STAGES + i); };
+  auto pfull = [&](int i) { return bars + 8u * (2 * STAGES + i); };        // partial sums written
+  auto pfree = [&](int i) { return bars + 8u * (2 * STAGES + 2 + i); };    // and read
+  const int tid = threadIdx.x, lane = tid & 31, warp = (int)uniform(tid >> 5), g = lane >> 2, q4 = lane & 3;
   const int T = A.T, H = A.H, I = A.I, E = A.E, K = A.K, G = (int)gridDim.x, cta = (int)blockIdx.x;
+  volatile int* abort_flag = &s_abort;
 
   // ------------------------------------------------------------------ who goes where
+  if (tid == THREADS - 1) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(full(i), 1);
+      mbar_init(empty(i), WARPS);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(pfull(i), WARPS);
+      mbar_init(pfree(i), FINISH);
+    }
+    s_abort = 0;
+    mbar_init_fence();
+  }
   for (int e = tid; e < E; e += THREADS) tab.mask[e] = 0;
   if (warp < T) {
     const float* row = A.logits + warp * E;
@@ -315,439 +356,523 @@ __global__ void __launch_bounds__(THREADS, 1) moe_small_layer(const SmallArgs A)
     else select_experts<MAX_E / 32>(row, E, K, A.renorm, lane, tab.ids + warp * MAX_K, tab.w + warp * MAX_K);
   }
   __syncthreads();
-  for (int i = tid; i < T * MAX_K; i += THREADS)
-    if (i % MAX_K < K) atomicOr(&tab.mask[tab.ids[i]], 1u << (i / MAX_K));
+  if (tid < T * MAX_K && lane < K) atomicOr(&tab.mask[tab.ids[tid]], 1u << warp);      // warp: the token
   __syncthreads();
   if (warp == 0) {
-    int n = 0, slots = 0;
+    int n = 0;
     for (int e0 = 0; e0 < E; e0 += 32) {
       const uint32_t m = e0 + lane < E ? tab.mask[e0 + lane] : 0u;
       const unsigned any = __ballot_sync(0xffffffffu, m != 0);
       const int at = n + __popc(any & ((1u << lane) - 1u));
-      int incl = __popc(m);
-      const int own = incl;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
       if (m != 0) {
         tab.hit[at] = (uint16_t)(e0 + lane);
         tab.pos[e0 + lane] = (uint16_t)at;
-        tab.before[at] = (uint16_t)(slots + incl - own);
+        tab.count[at] = (uint8_t)__popc(m);
       }
       n += __popc(any);
-      slots += __shfl_sync(0xffffffffu, incl, 31);
     }
     if (lane == 0) s_hits = n;
   }
   __syncthreads();
-  for (int i = tid; i < T * MAX_K; i += THREADS)
-    if (i % MAX_K < K) {
-      const int at = tab.pos[tab.ids[i]] * MAX_T + i / MAX_K;
-      tab.slot[at] = (uint8_t)(i % MAX_K);
-      tab.weight[at] = tab.w[i];
-    }
+  if (tid < T * MAX_K && lane < K) {
+    const int e = tab.ids[tid];
+    tab.slot[tab.pos[e] * MAX_T + __popc(tab.mask[e] & ((1u << warp) - 1u))] = (uint16_t)tid;
+  }
   __syncthreads();
   const int hits = s_hits;
+  auto row_of = [&](int slot) { return (slot >> 5) * K + (slot & 31); };   // row of h
+  static_assert(MAX_K == 32 && MAX_T * MAX_K <= THREADS, "a slot is a thread");
 
-  // ------------------------------------------------------------------ gate and up projections, SwiGLU
-  // The columns of h of all experts hit, one after the other, are cut into equal ranges (int4: by 16 columns).  A CTA walks
-  // its range in tiles; the warps share a tile's k (`ksplit` of them) and, where k is short, two or more tiles at a time.
-  // After `together` tiles the partial sums meet in shared memory (two buffers in turn, so one barrier a meeting).
-  {
-    const int64_t all = (int64_t)hits * (I / (W4 ? 16 : 1));
-    const int lo = (int)(all * cta / G) * (W4 ? 16 : 1), hi = (int)(all * (cta + 1) / G) * (W4 ? 16 : 1);
-    const int steps = (H + STEP - 1) / STEP, batches = (steps + BATCH - 1) / BATCH;
-    int ksplit = WARPS;
-    while (ksplit > batches) ksplit >>= 1;
-    const int at_once = WARPS / ksplit, together = PARTS / MT / ksplit, kw = warp % ksplit, tg = warp / ksplit;
-    struct Walk { int pos, place, end; } cur;      // column over all experts, the expert's place, where its columns end
-    cur.pos = lo;
-    cur.place = lo / I;
-    cur.end = (cur.place + 1) * I;
-    auto width = [&](const Walk& c) { return min(TW, min(c.end, hi) - c.pos); };
-    auto advance = [&](Walk& c) {
-      c.pos += width(c);
-      if (c.pos == c.end) { ++c.place; c.end += I; }
-    };
-    int tiles;                                     // of the whole range
-    {
-      const int p0 = lo / I, p1 = hi / I, r0 = lo - p0 * I, r1 = hi - p1 * I;
-      tiles = p0 == p1 ? (hi - lo + TW - 1) / TW
-                       : (I - r0 + TW - 1) / TW + (p1 - p0 - 1) * ((I + TW - 1) / TW) + (r1 + TW - 1) / TW;
-    }
-    uint4 a[BATCH][W4 ? 1 : 2], na[BATCH][W4 ? 1 : 2];      // row g / g + 8 pieces; int4: gate words, up words
-    uint2 sz[2], nsz[2];                                    // int4: scales of two columns, word of their zero points
-    auto fetch = [&](const Walk& c, int batch, uint4 (&d)[BATCH][W4 ? 1 : 2], uint2 (&dz)[2]) {
-      const size_t e = tab.hit[c.place];
-      const int col = c.pos - (c.end - I);
-      if (W4) {
-        const int k0 = batch * (BATCH * STEP), grp = k0 / A.group;
-        const size_t n = (size_t)col + 2 * g;
-#pragma unroll
-        for (int s = 0; s < BATCH; ++s) {
-          const size_t at = (e * (H / 8) + k0 / 8 + 4 * s + q4) * I + n;
-          const uint2 v0 = ld_weights2(A.qw[0] + at), v1 = ld_weights2(A.qw[1] + at);
-          d[s][0] = make_uint4(v0.x, v0.y, v1.x, v1.y);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const size_t row = e * (H / A.group) + grp;
-          dz[j].x = *reinterpret_cast<const uint32_t*>(A.sc[j] + row * I + n);
-          dz[j].y = (uint32_t)A.qz[j][row * (I / 8) + (n >> 3)] >> (4 * (n & 7));
-        }
-      } else {
-        const bool live = g < width(c);
-        const uint8_t* base = reinterpret_cast<const uint8_t*>(A.w13) + (e * 2 * I + col + g) * (size_t)H * SIZE;
-        const size_t up = (size_t)I * H * SIZE;
-#pragma unroll
-        for (int s = 0; s < BATCH; ++s) {
-          const int b = (batch * BATCH + s) * 64 + 16 * q4;
-          const bool in = live && b < H * SIZE;
-          d[s][0] = in ? ld_weights(base + b) : make_uint4(0u, 0u, 0u, 0u);
-          d[s][W4 ? 0 : 1] = in ? ld_weights(base + up + b) : make_uint4(0u, 0u, 0u, 0u);
-        }
-      }
-    };
-    for (int i = 0; i < tg && cur.pos < hi; ++i) advance(cur);
-    int index = tg;                                // of the warp's tile in the range
-    if (cur.pos < hi) fetch(cur, kw, a, sz);
-    const int meetings = (tiles + together - 1) / together;
-    for (int meet = 0; meet < meetings; ++meet) {
-      uint8_t* buf = part + (meet & 1) * PART_BUFFER * OCT;
-      while (index < tiles && index / together == meet) {
-        Walk nxt = cur;
-        for (int i = 0; i < at_once && nxt.pos < hi; ++i) advance(nxt);
-        const uint32_t mask = tab.mask[tab.hit[cur.place]];
-        Acc acc[OCT][MT][4] = {};
-        for (int batch = kw; batch < batches; batch += ksplit) {
-          if (batch + ksplit < batches) fetch(cur, batch + ksplit, na, nsz);
-          else if (nxt.pos < hi) fetch(nxt, kw, na, nsz);
-#pragma unroll
-          for (int o = 0; o < OCT; ++o) {
-            if (((mask >> (8 * o)) & 0xffu) == 0) continue;
-            const int tok = 8 * o + g;
-            float grp[MT][4] = {};
-#pragma unroll
-            for (int s = 0; s < BATCH; ++s) {
-              const int k = (batch * BATCH + s) * STEP + (16 / SIZE) * q4;
-              uint4 b = make_uint4(0u, 0u, 0u, 0u);
-              if (tok < T && k < H) {
-                const uint8_t* rows = F == F_INT8 ? reinterpret_cast<const uint8_t*>(A.xq) : reinterpret_cast<const uint8_t*>(A.x);
-                b = __ldg(reinterpret_cast<const uint4*>(rows + ((size_t)tok * H + k) * SIZE));
-              }
-              if constexpr (W4) {
-                b = pair_up(b);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                  const uint32_t z = sz[j].y;
-                  const float z0 = -(128.0f + (float)(z & 15u)), z1 = -(128.0f + (float)((z >> 4) & 15u));
-                  uint32_t v0[4], v1[4];
-                  unpack_int4(j == 0 ? a[s][0].x : a[s][0].z, __floats2bfloat162_rn(z0, z0), v0);
-                  unpack_int4(j == 0 ? a[s][0].y : a[s][0].w, __floats2bfloat162_rn(z1, z1), v1);
-                  mma_bf16(grp[j % MT], v0[0], v1[0], v0[1], v1[1], b.x, b.y);
-                  mma_bf16(grp[j % MT], v0[2], v1[2], v0[3], v1[3], b.z, b.w);
-                }
-              } else if constexpr (F == F_INT8) {
-                mma_s8(acc[o][0], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b.x, b.y);
-                mma_s8(acc[o][0], a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b.z, b.w);
-              } else if constexpr (F == F_F16) {
-                mma_f16(acc[o][0], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b.x, b.y);
-                mma_f16(acc[o][0], a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b.z, b.w);
-              } else {
-                mma_bf16(acc[o][0], a[s][0].x, a[s][1].x, a[s][0].y, a[s][1].y, b.x, b.y);
-                mma_bf16(acc[o][0], a[s][0].z, a[s][1].z, a[s][0].w, a[s][1].w, b.z, b.w);
-              }
-            }
-            if constexpr (W4) {                    // a batch lies inside a quantisation group
-#pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const float2 sc = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&sz[j].x));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[o][j][i] = fmaf(grp[j][i], i < 2 ? sc.x : sc.y, acc[o][j][i]);
-              }
-            }
-          }
-#pragma unroll
-          for (int s = 0; s < BATCH; ++s)
-#pragma unroll
-            for (int j = 0; j < (W4 ? 1 : 2); ++j) a[s][j] = na[s][j];
-          sz[0] = nsz[0];
-          sz[1] = nsz[1];
-        }
-        const int slot = index % together;
-#pragma unroll
-        for (int o = 0; o < OCT; ++o)
-#pragma unroll
-          for (int j = 0; j < MT; ++j) {
-            const Acc* c = acc[o][j];
-            *reinterpret_cast<int4*>(buf + ((((slot * ksplit + kw) * OCT + o) * MT + j) * 32 + lane) * 16) =
-                *reinterpret_cast<const int4*>(c);
-          }
-        if (kw == 0 && lane == 0) s_tile[meet & 1][slot] = make_int4(cur.place, cur.pos - (cur.end - I), width(cur), 0);
-        cur = nxt;
-        index += at_once;
-      }
-      __syncthreads();
-      // thread: a fragment position of a tile; its sums over the warps in order
-      for (int at_part = tid; at_part < together * OCT * 32; at_part += THREADS) {
-        const int slot = at_part / (OCT * 32), o = at_part / 32 % OCT;
-        if (meet * together + slot < tiles) {
-          const int4 tile = s_tile[meet & 1][slot];
-          const uint32_t mask = tab.mask[tab.hit[tile.x]];
-          if (((mask >> (8 * o)) & 0xffu) != 0) {
-            Acc sum[MT][4] = {};
-            for (int w = 0; w < ksplit; ++w)
-#pragma unroll
-              for (int j = 0; j < MT; ++j) {
-                const int4 raw = *reinterpret_cast<const int4*>(buf + ((((slot * ksplit + w) * OCT + o) * MT + j) * 32 + lane) * 16);
-                const Acc* c = reinterpret_cast<const Acc*>(&raw);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sum[j][i] += c[i];
-              }
-#pragma unroll
-            for (int i = 0; i < (W4 ? 4 : 2); ++i) {
-              const int tok = 8 * o + 2 * q4 + (i & 1), col = W4 ? 2 * g + (i >> 1) : g;
-              const bool live = ((mask >> tok) & 1u) != 0 && col < tile.z;
-              float v = 0.0f;
-              size_t at = 0;
-              if (live) {
-                at = (size_t)tok * K + tab.slot[tile.x * MAX_T + tok];
-                float gv, uv;
-                if constexpr (F == F_INT8) {
-                  const float* s = A.s13 + (size_t)tab.hit[tile.x] * 2 * I + tile.y + col;
-                  const float sx = A.xs[tok];
-                  gv = __fmul_rn(__fmul_rn(__int2float_rn(sum[0][i]), sx), s[0]);
-                  uv = __fmul_rn(__fmul_rn(__int2float_rn(sum[0][2 + i]), sx), s[I]);
-                } else {
-                  gv = (float)sum[0][i];
-                  uv = W4 ? (float)sum[MT - 1][i] : (float)sum[0][(2 + i) & 3];
-                }
-                const float p = expf(-fabsf(gv));
-                v = __fdividef(gv < 0.0f ? p * gv : gv, 1.0f + p) * uv;
-                if (F == F_BF16 || W4) {
-                  __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(A.h) + at * 2 * I + tile.y + col;
-                  const __nv_bfloat16 high = __float2bfloat16_rn(v);
-                  h[0] = high;
-                  h[I] = __float2bfloat16_rn(__hisinf(high) ? 0.0f : v - __bfloat162float(high));
-                } else {
-                  reinterpret_cast<float*>(A.h)[at * I + tile.y + col] = v;
-                }
-              }
-              if (F == F_INT8) {                   // the slot's largest |h|: first over the eight columns
-                uint32_t bits = abs_bits(v);
-#pragma unroll
-                for (int s = 4; s < 32; s <<= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, s));
-                if (g == 0 && ((mask >> tok) & 1u) != 0) atomicMax(A.amax + (size_t)tok * K + tab.slot[tile.x * MAX_T + tok], bits);
-              }
-            }
-          }
-        }
-      }
-    }
-  }
-
-  // ------------------------------------------------------------------ down projection: its weights on their way
-  // A CTA's output columns (rows of the down weights; int4: by 16), a tile of 16 at a time; its tasks are (expert, batch of
-  // k), dealt out to the warps.
+  // ------------------------------------------------------------------ the work
+  // Gate and up: the columns of h of all experts hit, one after the other, are cut into equal ranges (int4: by 16 columns).
+  // A CTA walks its range in tiles of A.tile columns; `ksplit` warps share a tile's k in units, so that `at_once` tiles are in
+  // work, for `passes` stages.  Down: a CTA's output columns (rows of the weights; int4: by 16), 16 at a time; the (expert,
+  // unit of k) pairs of a tile are dealt out to the warps in turn.
+  const int lo = W4 ? (int)((int64_t)hits * (I / 16) * cta / G) * 16 : (int)((int64_t)hits * I * cta / G);
+  const int hi = W4 ? (int)((int64_t)hits * (I / 16) * (cta + 1) / G) * 16 : (int)((int64_t)hits * I * (cta + 1) / G);
   const int out_lo = W4 ? (int)((int64_t)(H / 16) * cta / G) * 16 : (int)((int64_t)H * cta / G);
   const int out_hi = W4 ? (int)((int64_t)(H / 16) * (cta + 1) / G) * 16 : (int)((int64_t)H * (cta + 1) / G);
-  const int steps = (I + STEP - 1) / STEP, batches = (steps + BATCH - 1) / BATCH;
-  uint4 a[BATCH], c8[BATCH];                       // rows g and g + 8; int4: the words of two columns
-  uint2 sz;
-  auto fetch = [&](int row0, int task, uint4 (&d)[BATCH], uint4 (&d8)[BATCH], uint2& dz) {
-    const size_t e = tab.hit[task / batches];
-    const int batch = task % batches;
-    if (W4) {
-      const int k0 = batch * (BATCH * STEP);
-      const size_t n = (size_t)row0 + 2 * g, row = e * (I / A.group) + k0 / A.group;
-#pragma unroll
-      for (int s = 0; s < BATCH; ++s) {
-        const uint2 v = ld_weights2(A.qw[2] + (e * (I / 8) + k0 / 8 + 4 * s + q4) * H + n);
-        d[s].x = v.x;
-        d[s].y = v.y;
+  const int units = (H + UNIT_K - 1) / UNIT_K, units2 = (I + UNIT2_K - 1) / UNIT2_K;
+  const int TW = A.tile;
+  int tiles;
+  {
+    const int p0 = lo / I, p1 = hi / I, r0 = lo - p0 * I, r1 = hi - p1 * I;
+    tiles = p0 == p1 ? (hi - lo + TW - 1) / TW
+                     : (I - r0 + TW - 1) / TW + (p1 - p0 - 1) * ((I + TW - 1) / TW) + (r1 + TW - 1) / TW;
+  }
+  int ksplit = WARPS;
+  while (ksplit / 2 >= units) ksplit >>= 1;
+  const int at_once = WARPS / ksplit, passes = (units + ksplit - 1) / ksplit, rounds = (tiles + at_once - 1) / at_once;
+  const int tasks = hits * units2;
+  struct Walk { int pos, place, end; };            // column over all experts, the expert's place, where its columns end
+  auto width = [&](const Walk& c) { return min(TW, min(c.end, hi) - c.pos); };
+  auto next_tile = [&](Walk& c) {
+    c.pos += width(c);
+    if (c.pos == c.end) { ++c.place; c.end += I; }
+  };
+  auto skip_tiles = [&](Walk& c, int n) {
+    for (int i = 0; i < n && c.pos < hi; ++i) next_tile(c);
+  };
+  Walk walk;
+  walk.pos = lo;
+  walk.place = lo / I;
+  walk.end = (walk.place + 1) * I;
+
+  if (warp == WARPS + FINISH) {
+    // ------------------------------------------------------------------ copies: first gate and up, then down
+    // Weights only, so they run on through the barrier over the grid.  One elected lane issues, from uniform registers.
+    const bool leader = elect_one();
+    int stage = 0, filled = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    auto next_stage = [&] {
+      ++filled;
+      if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+    };
+    for (int round = 0; round < rounds && ok; ++round) {
+      for (int pass = 0; pass < passes && ok; ++pass) {
+        ok = mbar_wait_warp(empty(stage), phase ^ 1u, abort_flag, A.d_status);
+        if (!ok) break;
+        const int u0 = pass * ksplit, n = min(ksplit, units - u0), live = min(at_once, tiles - round * at_once);
+        const uint32_t dst = ring + stage * STAGE, bar = full(stage);
+        if (leader) mbar_expect_tx(bar, W4 ? live * 2 * A.box_rows * 64 : live * n * 2 * TW * 128);
+        Walk c = walk;
+        for (int i = 0; i < live; ++i) {
+          const int e = (int)uniform(tab.hit[c.place]), col = (int)uniform(c.pos - (c.end - I));
+          const uint32_t at = dst + i * ksplit * UNIT;
+          if (W4) {
+            if (leader) {
+              copy_box(at, &maps.gate, bar, col, u0 * 16, e);
+              copy_box(at + ksplit * (UNIT / 2), &maps.up, bar, col, u0 * 16, e);
+            }
+          } else {
+            for (int u = 0; u < n; ++u)
+              if (leader) copy_box(at + u * UNIT, &maps.gate, bar, (u0 + u) * UNIT_K, col, 0, e);
+          }
+          next_tile(c);
+        }
+        __syncwarp();
+        next_stage();
       }
-      dz.x = *reinterpret_cast<const uint32_t*>(A.sc[2] + row * H + n);
-      dz.y = (uint32_t)A.qz[2][row * (H / 8) + (n >> 3)] >> (4 * (n & 7));
-    } else {
-      const uint8_t* base = reinterpret_cast<const uint8_t*>(A.w2) + (e * H + row0 + g) * (size_t)I * SIZE;
-#pragma unroll
-      for (int s = 0; s < BATCH; ++s) {
-        const int b = (batch * BATCH + s) * 64 + 16 * q4;
-        const bool in = b < I * SIZE;
-        d[s] = in && row0 + g < out_hi ? ld_weights(base + b) : make_uint4(0u, 0u, 0u, 0u);
-        d8[s] = in && row0 + g + 8 < out_hi ? ld_weights(base + (size_t)8 * I * SIZE + b) : make_uint4(0u, 0u, 0u, 0u);
+      skip_tiles(walk, at_once);
+    }
+    for (int row0 = out_lo; row0 < out_hi && ok; row0 += 16) {
+      int place = 0, u = 0;
+      for (int task = 0; task < tasks && ok; task += WARPS) {
+        ok = mbar_wait_warp(empty(stage), phase ^ 1u, abort_flag, A.d_status);
+        if (!ok) break;
+        const int live = min(WARPS, tasks - task);
+        const uint32_t dst = ring + stage * STAGE, bar = full(stage);
+        if (leader) mbar_expect_tx(bar, live * (W4 ? UNIT : A.box_rows * 128));
+        for (int i = 0; i < live; ++i) {
+          const int e = (int)uniform(tab.hit[place]);
+          if (leader) {
+            if (W4) copy_box(dst + i * UNIT, &maps.down, bar, row0, u * 32, e);
+            else copy_box(dst + i * UNIT, &maps.down, bar, u * UNIT2_K, row0, e);
+          }
+          if (++u == units2) { u = 0; ++place; }
+        }
+        __syncwarp();
+        next_stage();
       }
     }
+    // nothing is on its way any more when the CTA ends
+    for (int f = max(0, filled - STAGES); f < filled; ++f)
+      mbar_wait_limited(full(f % STAGES), (uint32_t)(f / STAGES) & 1u, ok ? SPIN_LIMIT : 1u << 16);
+    return;
+  }
+
+  auto zero_pair = [](uint32_t z) {                // -(128 + z), twice
+    const float v = -(128.0f + (float)(z & 15u));
+    return __floats2bfloat162_rn(v, v);
   };
-  const int tasks = hits * batches;
-  if (out_lo < out_hi && warp < tasks) fetch(out_lo, warp, a, c8, sz);
+  // A lane's two 16-byte pieces of row `line` of a unit (rows of 128 bytes, swizzled by the copies).
+  auto piece = [&](const uint8_t* unit, int line, int s) {
+    return *reinterpret_cast<const uint4*>(unit + line * 128 + (((2 * q4 + s) ^ (line & 7)) << 4));
+  };
+  int stage = 0;
+  uint32_t phase = 0;
+  bool ok = true;                                  // a wait that ran out: the rest is walked through without waiting
+  auto release = [&] {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty(stage));
+    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+  };
+
+  if (warp < WARPS) {
+    // ------------------------------------------------------------------ gate and up projections
+    const int kw = warp % ksplit, tg = warp / ksplit;
+    skip_tiles(walk, tg);
+    const uint8_t* rows = F == F_INT8 ? reinterpret_cast<const uint8_t*>(A.xq) : reinterpret_cast<const uint8_t*>(A.x);
+    // x of the lane's token for a unit (column o * 8 + g of the expert); int4: the group's scales and zero points too
+    constexpr int XS = W4 ? 4 : 2;
+    auto load_x = [&](uint4 (&b)[XS], int place, int u, int o) {
+      const bool live = 8 * o + g < tab.count[place];
+      const uint8_t* row = rows + (size_t)(live ? tab.slot[place * MAX_T + 8 * o + g] >> 5 : 0) * H * SIZE;
+#pragma unroll
+      for (int s = 0; s < XS; ++s) {
+        const int k = W4 ? u * 256 + 64 * s + 16 * q4 : u * 128 + 32 * q4 + 16 * s;      // bytes
+        b[s] = live && k < H * SIZE ? __ldg(reinterpret_cast<const uint4*>(row + k)) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    };
+    auto load_sz = [&](uint32_t (&sz)[4], const Walk& c, int u) {
+      if constexpr (W4) {
+        const size_t n = (size_t)(c.pos - (c.end - I)) + 2 * g, row = (size_t)tab.hit[c.place] * (H / A.group) + u * 128 / A.group;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          sz[j] = __ldg(reinterpret_cast<const uint32_t*>(A.sc[j] + row * I + n));
+          sz[2 + j] = (uint32_t)__ldg(A.qz[j] + row * (I / 8) + (n >> 3)) >> (4 * (n & 7));
+        }
+      }
+    };
+    uint4 b[XS], nb[XS];
+    uint32_t sz[4] = {}, nsz[4] = {};
+    if (walk.pos < hi && kw < units) {
+      load_x(b, walk.place, kw, 0);
+      load_sz(sz, walk, kw);
+    }
+    for (int round = 0; round < rounds; ++round) {
+      const bool mine = walk.pos < hi;
+      Walk nxt = walk;
+      skip_tiles(nxt, at_once);
+      Acc acc[OCT][MT][4] = {};
+      for (int pass = 0; pass < passes; ++pass) {
+        const int u = pass * ksplit + kw;
+        // of the unit after this one
+        const bool last = pass + 1 == passes;
+        const Walk& c = last ? nxt : walk;
+        const int nu = last ? kw : u + ksplit;
+        if (c.pos < hi && nu < units) {
+          load_x(nb, c.place, nu, 0);
+          load_sz(nsz, c, nu);
+        }
+        if (ok) ok = mbar_wait_warp(full(stage), phase, abort_flag, A.d_status);
+        if (mine && u < units) {
+          const uint8_t* unit = small_smem + stage * STAGE + (W4 ? tg * ksplit * UNIT + kw * (UNIT / 2) : warp * UNIT);
+#pragma unroll
+          for (int o = 0; o < OCT; ++o) {
+            if (o == 1) {
+              if (tab.count[walk.place] <= 8) break;
+              load_x(b, walk.place, u, 1);
+            }
+            if constexpr (W4) {
+              float grp[MT][4] = {};
+#pragma unroll
+              for (int s = 0; s < 4; ++s) {
+                const uint4 x = pair_up(b[s]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                  const uint2 w = *reinterpret_cast<const uint2*>(unit + j * ksplit * (UNIT / 2) + (4 * s + q4) * 64 + 8 * g);
+                  uint32_t v0[4], v1[4];
+                  unpack_int4(w.x, zero_pair(sz[2 + j]), v0);
+                  unpack_int4(w.y, zero_pair(sz[2 + j] >> 4), v1);
+                  mma_bf16(grp[j % MT], v0[0], v1[0], v0[1], v1[1], x.x, x.y);
+                  mma_bf16(grp[j % MT], v0[2], v1[2], v0[3], v1[3], x.z, x.w);
+                }
+              }
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {        // a unit lies inside a quantisation group
+                const float2 sc = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&sz[j]));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[o][j % MT][i] = fmaf(grp[j % MT][i], i < 2 ? sc.x : sc.y, acc[o][j % MT][i]);
+              }
+            } else {
+#pragma unroll
+              for (int s = 0; s < 2; ++s) {
+                const uint4 r = piece(unit, g, s), r8 = piece(unit, TW + g, s);
+                if constexpr (F == F_INT8) {
+                  mma_s8(acc[o][0], r.x, r8.x, r.y, r8.y, b[s].x, b[s].y);
+                  mma_s8(acc[o][0], r.z, r8.z, r.w, r8.w, b[s].z, b[s].w);
+                } else if constexpr (F == F_F16) {
+                  mma_f16(acc[o][0], r.x, r8.x, r.y, r8.y, b[s].x, b[s].y);
+                  mma_f16(acc[o][0], r.z, r8.z, r.w, r8.w, b[s].z, b[s].w);
+                } else {
+                  mma_bf16(acc[o][0], r.x, r8.x, r.y, r8.y, b[s].x, b[s].y);
+                  mma_bf16(acc[o][0], r.z, r8.z, r.w, r8.w, b[s].z, b[s].w);
+                }
+              }
+            }
+          }
+        }
+        release();
+#pragma unroll
+        for (int s = 0; s < XS; ++s) b[s] = nb[s];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sz[j] = nsz[j];
+      }
+      const int buf = round & 1;
+      if (ok) ok = mbar_wait_warp(pfree(buf), ((round >> 1) & 1) ^ 1u, abort_flag, A.d_status);
+#pragma unroll
+      for (int o = 0; o < OCT; ++o)
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+          *reinterpret_cast<int4*>(part + buf * part_bytes(F, OCT) + (((warp * OCT + o) * MT + j) * 32 + lane) * 16) =
+              *reinterpret_cast<const int4*>(acc[o][j]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pfull(buf));
+      walk = nxt;
+    }
+  } else {
+    // ------------------------------------------------------------------ sums over the warps, SwiGLU
+    // A warp takes a tile's octet of tokens: a lane a fragment position, its sums over the warps in order.
+    for (int round = 0; round < rounds; ++round) {
+      const int buf = round & 1;
+      if (ok) ok = mbar_wait_warp(pfull(buf), (round >> 1) & 1, abort_flag, A.d_status);
+      const int live_tiles = min(at_once, tiles - round * at_once);
+      for (int slot = 0; slot < live_tiles; ++slot) {
+        const int place = walk.place, col0 = walk.pos - (walk.end - I), cols = width(walk);
+        next_tile(walk);
+        const size_t e = tab.hit[place];
+#pragma unroll
+        for (int o = 0; o < OCT; ++o) {
+          const int live = (int)tab.count[place] - 8 * o;                  // columns of this octet
+          if (live <= 0 || (slot * OCT + o) % FINISH != warp - WARPS) continue;
+          Acc sum[MT][4] = {};
+#pragma unroll 8
+          for (int w = 0; w < ksplit; ++w)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+              const int4 raw = *reinterpret_cast<const int4*>(part + buf * part_bytes(F, OCT) +
+                                                              ((((slot * ksplit + w) * OCT + o) * MT + j) * 32 + lane) * 16);
+              const Acc* c = reinterpret_cast<const Acc*>(&raw);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sum[j][i] += c[i];
+            }
+#pragma unroll
+          for (int i = 0; i < (W4 ? 4 : 2); ++i) {
+            const int n = 2 * q4 + (i & 1), col = W4 ? 2 * g + (i >> 1) : g;
+            float v = 0.0f;
+            const int code = n < live ? tab.slot[place * MAX_T + 8 * o + n] : 0;
+            const size_t row = row_of(code);
+            if (n < live && col < cols) {
+              float gv, uv;
+              if constexpr (F == F_INT8) {
+                const float* s = A.s13 + e * 2 * I + col0 + col;
+                const float sx = A.xs[code >> 5];
+                gv = __fmul_rn(__fmul_rn(__int2float_rn(sum[0][i]), sx), s[0]);
+                uv = __fmul_rn(__fmul_rn(__int2float_rn(sum[0][2 + i]), sx), s[I]);
+              } else {
+                gv = (float)sum[0][i];
+                uv = W4 ? (float)sum[MT - 1][i] : (float)sum[0][(2 + i) & 3];
+              }
+              const float p = expf(-fabsf(gv));
+              v = __fdividef(gv < 0.0f ? p * gv : gv, 1.0f + p) * uv;
+              if (F == F_BF16 || W4) {
+                __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(A.h) + row * 2 * I + col0 + col;
+                const __nv_bfloat16 high = __float2bfloat16_rn(v);
+                h[0] = high;
+                h[I] = __float2bfloat16_rn(__hisinf(high) ? 0.0f : v - __bfloat162float(high));
+              } else {
+                reinterpret_cast<float*>(A.h)[row * I + col0 + col] = v;
+              }
+            }
+            if (F == F_INT8) {                     // the row's largest |h|: first over the columns of the tile
+              uint32_t bits = abs_bits(v);
+#pragma unroll
+              for (int s = 4; s < 32; s <<= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, s));
+              if (g == 0 && n < live) atomicMax(A.amax + row, bits);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pfree(buf));
+    }
+  }
 
   // ------------------------------------------------------------------ every h is there
-  __syncthreads();
+  warps_meet<1, WARPS + FINISH>();
   if (tid == 0) {
-    __threadfence();
-    atomicAdd(A.counter, 1u);
-    uint32_t seen = 0, looks = 0;
-    do {
-      asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(A.counter) : "memory");
-    } while (seen < (unsigned)G && ++looks < POLL_LIMIT);
-    s_ok = seen >= (unsigned)G;
-    if (!s_ok && A.d_status != nullptr) atomicOr(A.d_status, (int)MQ_DEV_WAIT_EXPIRED);
-    __threadfence();
+    grid_arrive(A.counter);
+    s_ok = grid_wait(A.counter, (unsigned)G);
   }
-  __syncthreads();
-  if (!s_ok) return;
-
-  // ------------------------------------------------------------------ down projection and weighted sum
-  // int8: h is quantised here, by every CTA for itself.
-  int8_t* hq = reinterpret_cast<int8_t*>(part + 2 * SUM_BUFFER * OCT);
-  auto hq_row = [&](int place, uint32_t mask, int tok) {
-    return hq + (size_t)(tab.before[place] + __popc(mask & ((1u << tok) - 1u))) * (I + 16);
-  };
-  if (F == F_INT8) {
-    for (int i = warp; i < hits * MAX_T; i += WARPS) {
-      const int place = i / MAX_T, tok = i % MAX_T;
-      const uint32_t mask = tab.mask[tab.hit[place]];
-      if (((mask >> tok) & 1u) == 0) continue;
-      const size_t slot = (size_t)tok * K + tab.slot[i];
-      const RowScale r = row_scale(__ldcg(A.amax + slot));
-      const float* src = reinterpret_cast<const float*>(A.h) + slot * I;
-      int8_t* dst = hq_row(place, mask, tok);
+  warps_meet<1, WARPS + FINISH>();
+  if (F == F_INT8 && s_ok != 0) {                  // rows of h to int8, a warp a row over the whole grid, and a second barrier
+    for (int row = cta * WARPS + warp; row < T * K && warp < WARPS; row += G * WARPS) {
+      const RowScale r = row_scale(__ldcg(A.amax + row));
+      const float* src = reinterpret_cast<const float*>(A.h) + (size_t)row * I;
+#pragma unroll 4
       for (int k = 4 * lane; k < I; k += 128) {
         const float4 v = __ldcg(reinterpret_cast<const float4*>(src + k));
-        *reinterpret_cast<uint32_t*>(dst + k) =
+        *reinterpret_cast<uint32_t*>(A.hq + (size_t)row * I + k) =
             ((uint32_t)quantize(v.x, r) & 0xffu) | ((uint32_t)quantize(v.y, r) & 0xffu) << 8 |
             ((uint32_t)quantize(v.z, r) & 0xffu) << 16 | ((uint32_t)quantize(v.w, r) & 0xffu) << 24;
       }
     }
-    __syncthreads();
+    warps_meet<1, WARPS + FINISH>();
+    if (tid == 0) {
+      grid_arrive(A.counter);
+      s_ok = grid_wait(A.counter, 2u * (unsigned)G);
+    }
+    warps_meet<1, WARPS + FINISH>();
   }
-  int meet = 0;
+  if (warp >= WARPS) return;
+  if (s_ok == 0) {
+    if (tid == 0 && A.d_status != nullptr) atomicOr(A.d_status, (int)MQ_DEV_WAIT_EXPIRED);
+    return;
+  }
+
+  // ------------------------------------------------------------------ down projection and weighted sum
+  // A warp's sums of a tile, [tokens, 16 columns], are its own piece of shared memory, to which a unit's columns are added
+  // with their tokens' weights.  A token that did not choose the expert takes nothing from it, whatever its weights hold.
+  float* mine = reinterpret_cast<float*>(part) + warp * (128 * OCT);
+  constexpr int HS = 2;                            // steps that are loaded together; int4: a quarter of a unit
+  constexpr int QUARTERS = W4 ? 4 : 1;
+  auto load_h = [&](uint4 (&b)[HS][HP], int place, int u, int quarter, int o) {
+    const bool live = 8 * o + g < tab.count[place];
+    const size_t row = live ? row_of(tab.slot[place * MAX_T + 8 * o + g]) : 0;
+#pragma unroll
+    for (int s = 0; s < HS; ++s) {
+      const int k = W4 ? u * UNIT2_K + 64 * quarter + 32 * s + 8 * q4 : u * UNIT2_K + (32 / SIZE) * q4 + (16 / SIZE) * s;
+      const bool in = live && k < I;
+#pragma unroll
+      for (int p = 0; p < HP; ++p) {
+        b[s][p] = make_uint4(0u, 0u, 0u, 0u);
+        if (in) {
+          const uint8_t* src;
+          if (F == F_INT8) src = reinterpret_cast<const uint8_t*>(A.hq) + row * I + k;
+          else if (F == F_F16) src = reinterpret_cast<const uint8_t*>(A.h) + (row * I + k) * 4 + 16 * p;
+          else src = reinterpret_cast<const uint8_t*>(A.h) + ((row * 2 + p) * I + k) * 2;
+          b[s][p] = __ldcg(reinterpret_cast<const uint4*>(src));
+        }
+      }
+    }
+  };
+  uint4 b[HS][HP], nb[HS][HP];
+  int place = warp / units2, u = warp - place * units2;
+  const int step_place = WARPS / units2, step_u = WARPS - step_place * units2;
+  if (warp < tasks) load_h(b, place, u, 0, 0);
   for (int row0 = out_lo; row0 < out_hi; row0 += 16) {
-    float sum[OCT][4] = {};
-    for (int task = warp; task < tasks; task += WARPS) {
-      uint4 na[BATCH], nc8[BATCH];
-      uint2 nsz;
-      const bool more = task + WARPS < tasks, next_tile = !more && row0 + 16 < out_hi;
-      if (more) fetch(row0, task + WARPS, na, nc8, nsz);
-      else if (next_tile) fetch(row0 + 16, warp, na, nc8, nsz);
-      const int place = task / batches, batch = task % batches;
-      const uint32_t mask = tab.mask[tab.hit[place]];
+    for (int i = lane; i < 128 * OCT; i += 32) mine[i] = 0.0f;
+    __syncwarp();
+    for (int task = warp; task - warp < tasks; task += WARPS) {
+      int np = place + step_place, nu = u + step_u;
+      if (nu >= units2) { nu -= units2; ++np; }
+      const bool live_task = task < tasks;
+      if (task + WARPS >= tasks) {                 // the next tile's first
+        np = warp / units2;
+        nu = warp - np * units2;
+      }
+      uint32_t sc[2] = {}, zp[2] = {};
+      if constexpr (W4) {
+        if (live_task) {
 #pragma unroll
-      for (int o = 0; o < OCT; ++o) {
-        if (((mask >> (8 * o)) & 0xffu) == 0) continue;
-        const int tok = 8 * o + g;
-        const bool live = ((mask >> tok) & 1u) != 0;
-        const size_t slot = live ? (size_t)tok * K + tab.slot[place * MAX_T + tok] : 0;
-        Acc acc[4] = {};
+          for (int j = 0; j < 2; ++j) {
+            const size_t n = (size_t)row0 + 2 * g, row = (size_t)tab.hit[place] * (I / A.group) + min(u * 256 + 128 * j, I - 1) / A.group;
+            sc[j] = __ldg(reinterpret_cast<const uint32_t*>(A.sc[2] + row * H + n));
+            zp[j] = (uint32_t)__ldg(A.qz[2] + row * (H / 8) + (n >> 3)) >> (4 * (n & 7));
+          }
+        }
+      }
+      if (ok) ok = mbar_wait_warp(full(stage), phase, abort_flag, A.d_status);
+      const uint8_t* unit = small_smem + stage * STAGE + warp * UNIT;
+      if (live_task) {
+        Acc acc[OCT][4] = {};
+        const bool second = OCT == 2 && tab.count[place] > 8;
 #pragma unroll
-        for (int s = 0; s < BATCH; ++s) {
-          const int k = (batch * BATCH + s) * STEP + (16 / SIZE) * q4;
-          const bool in = live && k < I;
-          if constexpr (F == F_INT8) {
-            uint4 b = make_uint4(0u, 0u, 0u, 0u);
-            if (in) b = *reinterpret_cast<const uint4*>(hq_row(place, mask, tok) + k);
-            mma_s8(acc, a[s].x, c8[s].x, a[s].y, c8[s].y, b.x, b.y);
-            mma_s8(acc, a[s].z, c8[s].z, a[s].w, c8[s].w, b.z, b.w);
-          } else if constexpr (F == F_F16) {
-            float4 f[2] = {};
-            if (in) {
-              const float4* src = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(A.h) + slot * I + k);
-              f[0] = __ldcg(src);
-              f[1] = __ldcg(src + 1);
+        for (int quarter = 0; quarter < QUARTERS; ++quarter) {
+          if (quarter + 1 < QUARTERS) load_h(nb, place, u, quarter + 1, 0);
+          else if (np < hits) load_h(nb, np, nu, 0, 0);
+#pragma unroll
+          for (int o = 0; o < OCT; ++o) {
+            if (o == 1) {
+              if (!second) break;
+              load_h(b, place, u, quarter, 1);
             }
-            const float* v = reinterpret_cast<const float*>(f);
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(&a[s]);
-            const uint32_t* w8 = reinterpret_cast<const uint32_t*>(&c8[s]);
+            float grp[4] = {};
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
-              // a tf32 number is the upper 19 bits of an fp32 one; fp16 fits, h is a sum of two
-              const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&w[p]));
-              const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&w8[p]));
-              const uint32_t h0 = __float_as_uint(v[2 * p]) & 0xffffe000u, h1 = __float_as_uint(v[2 * p + 1]) & 0xffffe000u;
-              const uint32_t l0 = isinf(v[2 * p]) ? 0u : __float_as_uint(v[2 * p] - __uint_as_float(h0)) & 0xffffe000u;
-              const uint32_t l1 = isinf(v[2 * p + 1]) ? 0u : __float_as_uint(v[2 * p + 1] - __uint_as_float(h1)) & 0xffffe000u;
-              const uint32_t a0 = __float_as_uint(lo.x), a1 = __float_as_uint(hi.x), a2 = __float_as_uint(lo.y), a3 = __float_as_uint(hi.y);
-              mma_tf32(acc, a0, a1, a2, a3, l0, l1);
-              mma_tf32(acc, a0, a1, a2, a3, h0, h1);
-            }
-          } else {
-            uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
-            if (in) {
-              const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(A.h) + slot * 2 * I + k;
-              hi = __ldcg(reinterpret_cast<const uint4*>(src));
-              lo = __ldcg(reinterpret_cast<const uint4*>(src + I));
+            for (int s = 0; s < HS; ++s) {
+              if constexpr (W4) {
+                const uint4 hi4 = pair_up(b[s][0]), lo4 = pair_up(b[s][HP - 1]);
+                const uint2 w = *reinterpret_cast<const uint2*>(unit + (8 * quarter + 4 * s + q4) * 64 + 8 * g);
+                uint32_t v0[4], v1[4];
+                unpack_int4(w.x, zero_pair(zp[quarter / 2]), v0);
+                unpack_int4(w.y, zero_pair(zp[quarter / 2] >> 4), v1);
+                mma_bf16(grp, v0[0], v1[0], v0[1], v1[1], lo4.x, lo4.y);
+                mma_bf16(grp, v0[2], v1[2], v0[3], v1[3], lo4.z, lo4.w);
+                mma_bf16(grp, v0[0], v1[0], v0[1], v1[1], hi4.x, hi4.y);
+                mma_bf16(grp, v0[2], v1[2], v0[3], v1[3], hi4.z, hi4.w);
+              } else {
+                const uint4 r4 = piece(unit, g, s), r84 = piece(unit, 8 + g, s);
+                if constexpr (F == F_INT8) {
+                  const uint4 x = b[s][0];
+                  mma_s8(acc[o], r4.x, r84.x, r4.y, r84.y, x.x, x.y);
+                  mma_s8(acc[o], r4.z, r84.z, r4.w, r84.w, x.z, x.w);
+                } else if constexpr (F == F_F16) {
+                  const uint32_t r[4] = {r4.x, r4.y, r4.z, r4.w}, r8[4] = {r84.x, r84.y, r84.z, r84.w};
+                  const uint32_t x[8] = {b[s][0].x, b[s][0].y, b[s][0].z, b[s][0].w, b[s][HP - 1].x, b[s][HP - 1].y, b[s][HP - 1].z, b[s][HP - 1].w};
+#pragma unroll
+                  for (int p = 0; p < 4; ++p) {
+                    // a tf32 number is the upper 19 bits of an fp32 one: fp16 fits, h is a sum of two
+                    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r[p]));
+                    const float2 a8 = __half22float2(*reinterpret_cast<const __half2*>(&r8[p]));
+                    const float v0 = __uint_as_float(x[2 * p]), v1 = __uint_as_float(x[2 * p + 1]);
+                    const uint32_t h0 = x[2 * p] & 0xffffe000u, h1 = x[2 * p + 1] & 0xffffe000u;
+                    const uint32_t l0 = isinf(v0) ? 0u : __float_as_uint(v0 - __uint_as_float(h0)) & 0xffffe000u;
+                    const uint32_t l1 = isinf(v1) ? 0u : __float_as_uint(v1 - __uint_as_float(h1)) & 0xffffe000u;
+                    const uint32_t a0 = __float_as_uint(a.x), a1 = __float_as_uint(a8.x), a2 = __float_as_uint(a.y), a3 = __float_as_uint(a8.y);
+                    mma_tf32(acc[o], a0, a1, a2, a3, l0, l1);
+                    mma_tf32(acc[o], a0, a1, a2, a3, h0, h1);
+                  }
+                } else {
+                  const uint4 h4 = b[s][0], l4 = b[s][HP - 1];
+                  mma_bf16(acc[o], r4.x, r84.x, r4.y, r84.y, l4.x, l4.y);
+                  mma_bf16(acc[o], r4.z, r84.z, r4.w, r84.w, l4.z, l4.w);
+                  mma_bf16(acc[o], r4.x, r84.x, r4.y, r84.y, h4.x, h4.y);
+                  mma_bf16(acc[o], r4.z, r84.z, r4.w, r84.w, h4.z, h4.w);
+                }
+              }
             }
             if constexpr (W4) {
-              hi = pair_up(hi);
-              lo = pair_up(lo);
-              const float z0 = -(128.0f + (float)(sz.y & 15u)), z1 = -(128.0f + (float)((sz.y >> 4) & 15u));
-              uint32_t v0[4], v1[4];
-              unpack_int4(a[s].x, __floats2bfloat162_rn(z0, z0), v0);
-              unpack_int4(a[s].y, __floats2bfloat162_rn(z1, z1), v1);
-              mma_bf16(acc, v0[0], v1[0], v0[1], v1[1], lo.x, lo.y);
-              mma_bf16(acc, v0[2], v1[2], v0[3], v1[3], lo.z, lo.w);
-              mma_bf16(acc, v0[0], v1[0], v0[1], v1[1], hi.x, hi.y);
-              mma_bf16(acc, v0[2], v1[2], v0[3], v1[3], hi.z, hi.w);
-            } else {
-              mma_bf16(acc, a[s].x, c8[s].x, a[s].y, c8[s].y, lo.x, lo.y);
-              mma_bf16(acc, a[s].z, c8[s].z, a[s].w, c8[s].w, lo.z, lo.w);
-              mma_bf16(acc, a[s].x, c8[s].x, a[s].y, c8[s].y, hi.x, hi.y);
-              mma_bf16(acc, a[s].z, c8[s].z, a[s].w, c8[s].w, hi.z, hi.w);
+              const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&sc[quarter / 2]));
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[o][i] = fmaf(grp[i], i < 2 ? f.x : f.y, acc[o][i]);
+            }
+          }
+#pragma unroll
+          for (int s = 0; s < HS; ++s)
+#pragma unroll
+            for (int p = 0; p < HP; ++p) b[s][p] = nb[s][p];
+        }
+#pragma unroll
+        for (int o = 0; o < OCT; ++o) {
+          const int live = (int)tab.count[place] - 8 * o;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int n = 2 * q4 + (i & 1);
+            if (n < live) {
+              const int slot = tab.slot[place * MAX_T + 8 * o + n];
+              const int col = W4 ? 2 * g + (i >> 1) : g + 8 * (i >> 1);
+              float v = (float)acc[o][i];
+              if (F == F_INT8)
+                v = v * scale_of(__ldcg(A.amax + row_of(slot))) *
+                    (row0 + col < out_hi ? A.s2[(size_t)tab.hit[place] * H + row0 + col] : 0.0f);
+              float* to = mine + (slot >> 5) * 16 + col;
+              *to = fmaf(v, tab.w[slot], *to);
             }
           }
         }
-        // into the tokens' sums; a token that did not choose the expert takes nothing from it, whatever its weights hold
-        float s0 = 1.0f, s1 = 1.0f;
-        if constexpr (W4) {
-          const float2 sc = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&sz.x));
-          s0 = sc.x;
-          s1 = sc.y;
-        } else if constexpr (F == F_INT8) {
-          const float* s = A.s2 + (size_t)tab.hit[place] * H + row0 + g;
-          s0 = row0 + g < out_hi ? s[0] : 0.0f;
-          s1 = row0 + g + 8 < out_hi ? s[8] : 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tk = 8 * o + 2 * q4 + (i & 1);
-          if (((mask >> tk) & 1u) == 0) continue;
-          float v = (float)acc[i];
-          if (F == F_INT8) v *= scale_of(__ldcg(A.amax + (size_t)tk * K + tab.slot[place * MAX_T + tk]));
-          if (F == F_INT8 || W4) v *= i < 2 ? s0 : s1;
-          sum[o][i] = fmaf(v, tab.weight[place * MAX_T + tk], sum[o][i]);
-        }
+      } else if (np < hits) {
+        load_h(b, np, nu, 0, 0);
       }
-      if (more || next_tile) {
-#pragma unroll
-        for (int s = 0; s < BATCH; ++s) {
-          a[s] = na[s];
-          c8[s] = nc8[s];
-        }
-        sz = nsz;
-      }
+      release();
+      place = np;
+      u = nu;
     }
+    warps_meet<2, WARPS>();
     // the warps' sums, in order, then the one rounding
-    float4* buf = reinterpret_cast<float4*>(part + (meet & 1) * SUM_BUFFER * OCT);
-    meet ^= 1;
-#pragma unroll
-    for (int o = 0; o < OCT; ++o)
-      buf[(warp * OCT + o) * 32 + lane] = make_float4(sum[o][0], sum[o][1], sum[o][2], sum[o][3]);
-    __syncthreads();
-    if (tid < OCT * 128) {                         // tid: (octet, register, lane of the fragment)
-      const int o = tid / 128, i = tid / 32 % 4;
+    if (tid < 128 * OCT) {
       float v = 0.0f;
-      for (int w = 0; w < WARPS; ++w) v += reinterpret_cast<const float*>(&buf[(w * OCT + o) * 32 + lane])[i];
-      const int tok = 8 * o + 2 * q4 + (i & 1);
-      const int row = row0 + (W4 ? 2 * g + (i >> 1) : g + 8 * (i >> 1));
-      if (tok < T && row < out_hi) {
-        const size_t at = (size_t)tok * H + row;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) v += reinterpret_cast<const float*>(part)[w * (128 * OCT) + tid];
+      const int tok = tid / 16, col = row0 + tid % 16;
+      if (tok < T && col < out_hi) {
+        const size_t at = (size_t)tok * H + col;
         if (A.residual != nullptr) v += to_float<OutT>(reinterpret_cast<const OutT*>(A.residual)[at]);
         reinterpret_cast<OutT*>(A.out)[at] = from_float<OutT>(v);
       }
     }
+    if (row0 + 16 < out_hi) warps_meet<2, WARPS>();
   }
 }
 
@@ -765,9 +890,7 @@ bool shape_ok(const mq_moe_layer& L, int64_t T) {
   if (E * 2 * I >= ((int64_t)1 << 31)) return false;
   switch (format_of(L)) {
     case F_INT4: return L.group_size % 128 == 0 && H % L.group_size == 0 && I % L.group_size == 0 && L.dtype == MQ_BF16;
-    case F_INT8:                                   // the quantised h of all slots lies in shared memory
-      return H % 16 == 0 && I % 16 == 0 && H <= 131071 &&
-             front_bytes(true, T <= 8 ? 1 : 2, T * K, I) + Tables::bytes((int)T, (int)E, (int)K) <= SMEM_LIMIT;
+    case F_INT8: return H % 16 == 0 && I % 16 == 0 && H <= 131071 && I <= 131071;
     default: return L.dtype != MQ_F32 && H % 8 == 0 && I % 8 == 0;
   }
 }
@@ -785,7 +908,9 @@ size_t carve_small(const mq_moe_layer& L, int64_t T, uint8_t* base, SmallArgs& A
   A.logits = (float*)take((size_t)(T * L.experts) * 4);
   A.xs = (float*)take((size_t)T * 4);
   A.h = take(S * (size_t)L.inter * 4);
-  A.xq = format_of(L) == F_INT8 ? (int8_t*)take((size_t)(T * L.hidden)) : nullptr;
+  const bool int8 = format_of(L) == F_INT8;
+  A.xq = int8 ? (int8_t*)take((size_t)(T * L.hidden)) : nullptr;
+  A.hq = int8 ? (int8_t*)take(S * (size_t)L.inter) : nullptr;
   return used;
 }
 
@@ -794,16 +919,60 @@ bool small_layer_ok(const mq_moe_layer* L) {
          valid_dtype(L->dtype) && valid_dtype(L->router_dtype) && !(L->int8_experts && L->group_size > 0);
 }
 
+bool small_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank, const cuuint64_t* dims,
+               const cuuint64_t* strides, const cuuint32_t* box, bool swizzle) {
+  EncodeTiledFn fn = tensor_map_encoder();
+  const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  return fn && fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Chooses the tile shapes and describes the weights to the copies.
+template <int F>
+bool small_maps(SmallArgs& A, int sms, SmallMaps& m) {
+  const cuuint64_t H = (cuuint64_t)A.H, I = (cuuint64_t)A.I, E = (cuuint64_t)A.E;
+  if constexpr (F == F_INT4) {
+    A.tile = 16;
+    A.box_rows = A.H / 8 < 256 ? A.H / 8 : 256;
+    const cuuint64_t in_dims[3] = {I, H / 8, E}, in_strides[2] = {I * 4, I * (H / 8) * 4};
+    const cuuint64_t out_dims[3] = {H, I / 8, E}, out_strides[2] = {H * 4, H * (I / 8) * 4};
+    const cuuint32_t in_box[3] = {16, (cuuint32_t)A.box_rows, 1}, out_box[3] = {16, 32, 1};
+    return small_map(&m.gate, CU_TENSOR_MAP_DATA_TYPE_INT32, A.qw[0], 3, in_dims, in_strides, in_box, false) &&
+           small_map(&m.up, CU_TENSOR_MAP_DATA_TYPE_INT32, A.qw[1], 3, in_dims, in_strides, in_box, false) &&
+           small_map(&m.down, CU_TENSOR_MAP_DATA_TYPE_INT32, A.qw[2], 3, out_dims, out_strides, out_box, false);
+  } else {
+    constexpr int SIZE = Fmt<F>::SIZE;
+    const CUtensorMapDataType type = F == F_INT8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                     : F == F_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    // one token hits top_k experts: the tiles of a CTA's share can be made equal
+    A.tile = 8;
+    if (A.T == 1) {
+      const int share = (int)(((int64_t)A.K * A.I + sms - 1) / sms), n = (share + 7) / 8;
+      A.tile = (share + n - 1) / n;
+    }
+    const int rows = (A.H + sms - 1) / sms;
+    A.box_rows = rows < 16 ? rows : 16;
+    const cuuint64_t in_dims[4] = {H, I, 2, E}, in_strides[3] = {H * SIZE, I * H * SIZE, 2 * I * H * SIZE};
+    const cuuint64_t out_dims[3] = {I, H, E}, out_strides[2] = {I * SIZE, H * I * SIZE};
+    const cuuint32_t in_box[4] = {128 / SIZE, (cuuint32_t)A.tile, 2, 1}, out_box[3] = {128 / SIZE, (cuuint32_t)A.box_rows, 1};
+    return small_map(&m.gate, type, A.w13, 4, in_dims, in_strides, in_box, true) &&
+           small_map(&m.down, type, A.w2, 3, out_dims, out_strides, out_box, true);
+  }
+}
+
 template <int F, int OCT, typename OutT>
 int launch_layer(const SmallArgs& A, cudaStream_t st) {
-  const size_t smem = front_bytes(F == F_INT8, OCT, A.T * A.K, A.I) + Tables::bytes(A.T, A.E, A.K);
+  const size_t smem = front_bytes(F, OCT) + Tables::bytes(A.T, A.E, A.K) + 1024;
   cudaError_t e = cudaFuncSetAttribute(moe_small_layer<F, OCT, OutT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   int dev = 0, sms = 0;
   if (e == cudaSuccess) e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess) {
     SmallArgs args = A;
-    void* argv[] = {&args};
+    SmallMaps maps = {};
+    if (!small_maps<F>(args, sms, maps)) return MQ_ERR_DRIVER_ENTRY;
+    void* argv[] = {&args, &maps};
     e = cudaLaunchCooperativeKernel((const void*)moe_small_layer<F, OCT, OutT>, dim3(sms), dim3(THREADS), argv, smem, st);
   }
   if (e != cudaSuccess) {

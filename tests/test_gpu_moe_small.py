@@ -242,7 +242,7 @@ def test_refusals():
     big = _cabi.MoELayer(hidden=128, inter=16384, experts=8, top_k=8, dtype=1, router_dtype=1, int8_experts=1)
     import ctypes
     lib = _cabi.load()
-    assert lib.mq_moe_small_covers(ctypes.addressof(big), 1) == 1 and lib.mq_moe_small_covers(ctypes.addressof(big), 16) == 0
+    assert lib.mq_moe_small_covers(ctypes.addressof(big), 16) == 1 and lib.mq_moe_small_covers(ctypes.addressof(big), 17) == 0
     # a workspace that is too small, or not there, is refused before any launch
     big.inter, big.int8_experts = 128, 0
     big.router, big.gate[0], big.down[0] = lay.router.data_ptr(), lay.w13.data_ptr(), lay.w2.data_ptr()
