@@ -18,8 +18,8 @@ __device__ __forceinline__ float scale_of(uint32_t max_bits) {
   return __fdiv_rn(__uint_as_float(max_bits), 127.0f);
 }
 
-// What a row's values are multiplied by on their way to q: 0 for rows without values to scale.  Scales below 2^-120 have
-// a reciprocal out of range or too coarse; those rows divide (quantize() below, exact = true).
+// What a row's values are multiplied by on their way to q; 0 for rows without values to scale.  Scales below 2^-120 have a
+// reciprocal out of range or too coarse; those rows divide (exact).
 struct RowScale {
   float scale, inv;
   bool exact;
@@ -32,15 +32,44 @@ __device__ __forceinline__ RowScale row_scale(uint32_t max_bits) {
   return r;
 }
 
-// x * inv is off by less than 2e-5 (|q| <= 127.5, three roundings of 2^-24), so it names the nearest whole number unless
-// it lies within 1e-4 of a half.  There, and for tiny scales, the quotient is taken in 64 bits, where it is a half only
-// if it is exactly one.
+// The quotient in 64 bits, where it is a half only if it is exactly one (out of line: it is rare, and long).
+static __device__ __noinline__ int exact_quotient(float x, float scale) {
+  return (int)fmin(fmax(rint(__ddiv_rn((double)x, (double)scale)), -127.0), 127.0);
+}
+
+// N values to bytes.  1.5 * 2^23 + x * inv, rounded once, has the nearest whole number in its low bits.  x * inv is off the
+// quotient by |q| 2^-24 < 8e-6 at most, so the number is the right one unless x * inv lies within 1.6e-5 of a half; there
+// the quotient is taken exactly.  No clamp: |x| * inv <= 127 (1 + 2^-22).
+template <int N>
+__device__ __forceinline__ void quantize(const float (&x)[N], const RowScale& r, uint32_t (&q)[N / 4]) {
+  constexpr float MAGIC = 12582912.0f;
+  uint32_t y[N];
+  float off = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float v = __fmaf_rn(x[i], r.inv, MAGIC);
+    y[i] = __float_as_uint(v);
+    off = fmaxf(off, fabsf(__fmaf_rn(x[i], r.inv, __fsub_rn(MAGIC, v))));
+  }
+  if (r.inv == 0.0f && !r.exact) {                               // zeros, or no numbers
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = 0u;
+  } else if (r.exact || off > 0.499984f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float d = r.exact ? 1.0f : fabsf(__fmaf_rn(x[i], r.inv, MAGIC - __uint_as_float(y[i])));
+      if (d > 0.499984f) y[i] = (uint32_t)exact_quotient(x[i], r.scale);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N / 4; ++i)
+    q[i] = __byte_perm(__byte_perm(y[4 * i], y[4 * i + 1], 0x0040), __byte_perm(y[4 * i + 2], y[4 * i + 3], 0x0040), 0x5410);
+}
 __device__ __forceinline__ int quantize(float x, const RowScale& r) {
-  if (r.inv == 0.0f && !r.exact) return 0;                       // nothing to scale
-  const float v = __fmul_rn(x, r.inv);
-  float q = rintf(v);
-  if (r.exact || fabsf(v - q) > 0.4999f) q = (float)rint(__ddiv_rn((double)x, (double)r.scale));
-  return (int)fminf(fmaxf(q, -127.0f), 127.0f);
+  const float v[4] = {x, 0.0f, 0.0f, 0.0f};
+  uint32_t q[1];
+  quantize<4>(v, r, q);
+  return (int)(int8_t)(q[0] & 0xffu);
 }
 
 }  // namespace int8

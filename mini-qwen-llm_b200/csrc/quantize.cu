@@ -1,6 +1,8 @@
-// Int8 rows for the W8A8 products (int8.cuh has the arithmetic).  One pass: a warp keeps its row in registers between
-// the maximum and the quotients (rows of up to 8 KB); longer rows are read a second time, from L2.
+// Int8 rows for the W8A8 products (int8.cuh has the arithmetic).  One pass: a warp (rows of up to 2 KB) or a CTA keeps its row
+// in registers between the maximum and the quotients; rows of over 32 KB, or off the 16-byte grid, are read a second time.
 // Bound by HBM: size + 1 bytes per element.
+#include <string.h>
+
 #include "int8.cuh"
 
 namespace mq {
@@ -10,44 +12,64 @@ using namespace int8;
 
 __device__ __forceinline__ uint32_t warp_max(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
-// The row's 16-byte vectors i * 32 + lane, NV a lane.
+// The largest magnitude of a lane's vectors, as the bits of an fp32 number.  16-bit numbers are compared two at a time, as
+// integers.
 template <typename T, int NV>
+__device__ __forceinline__ uint32_t largest(const uint4 (&v)[NV]) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (sizeof(T) == 4) top = max(top, w[j] & 0x7fffffffu);
+      else top = __vmaxu2(top, w[j] & 0x7fff7fffu);
+    }
+  }
+  if (sizeof(T) == 4) return top;
+  const uint16_t one = (uint16_t)max(top & 0xffffu, top >> 16);
+  T value;
+  memcpy(&value, &one, sizeof(one));
+  return abs_bits(to_float<T>(value));
+}
+
+// TPR threads a row, NV of its 16-byte vectors each: a warp a row, or a CTA of 256.
+template <typename T, int NV, int TPR>
 __global__ void __launch_bounds__(256)
 quantize_rows(const T* __restrict__ x, int64_t stride, int64_t rows, int K, int8_t* __restrict__ q, float* __restrict__ scale) {
   constexpr int V = 16 / sizeof(T);
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (row >= rows) return;
+  const int at = (int)threadIdx.x % TPR;
+  const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  if (TPR == 32 && row >= rows) return;
   const int nvec = K / V;
   const uint4* src = reinterpret_cast<const uint4*>(x + row * stride);
   uint4 v[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int p = i * 32 + lane;
+    const int p = i * TPR + at;
     v[i] = p < nvec ? src[p] : make_uint4(0u, 0u, 0u, 0u);
   }
-  uint32_t top = 0;
+  uint32_t top = warp_max(largest<T, NV>(v));
+  if (TPR == 256) {
+    __shared__ uint32_t part[8];
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const T* e = reinterpret_cast<const T*>(&v[i]);
-#pragma unroll
-    for (int j = 0; j < V; ++j) top = max(top, abs_bits(to_float<T>(e[j])));
+    for (int i = 0; i < 8; ++i) top = max(top, part[i]);
   }
-  const RowScale r = row_scale(warp_max(top));
-  if (lane == 0) scale[row] = r.scale;
+  const RowScale r = row_scale(top);
+  if (at == 0) scale[row] = r.scale;
   int8_t* dst = q + row * K;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int p = i * 32 + lane;
+    const int p = i * TPR + at;
     if (p < nvec) {
       const T* e = reinterpret_cast<const T*>(&v[i]);
+      float f[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = to_float<T>(e[j]);
       uint32_t w[V / 4];
-#pragma unroll
-      for (int j = 0; j < V / 4; ++j) {
-        w[j] = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) w[j] |= ((uint32_t)quantize(to_float<T>(e[4 * j + b]), r) & 0xffu) << (8 * b);
-      }
+      quantize<V>(f, r, w);
       if (V == 8) *reinterpret_cast<uint2*>(dst + p * 8) = make_uint2(w[0], w[V / 4 - 1]);
       else *reinterpret_cast<uint32_t*>(dst + p * 4) = w[0];
     }
@@ -78,15 +100,17 @@ int launch_quantize(const void* x, int64_t rows, int64_t K, int64_t stride, int8
   constexpr int V = 16 / sizeof(T);
   const T* xs = reinterpret_cast<const T*>(x);
   const int64_t nvec = K / V;
-  if (K % V == 0 && stride % V == 0 && aligned16(x) && (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && nvec <= 32 * 16) {
-    const unsigned blocks = (unsigned)((rows + 7) / 8);
-#define MQ_QUANTIZE(NV) quantize_rows<T, NV><<<blocks, 256, 0, st>>>(xs, stride, rows, (int)K, q, scale)
-    if (nvec <= 32) MQ_QUANTIZE(1);
-    else if (nvec <= 32 * 2) MQ_QUANTIZE(2);
-    else if (nvec <= 32 * 3) MQ_QUANTIZE(3);
-    else if (nvec <= 32 * 4) MQ_QUANTIZE(4);
-    else if (nvec <= 32 * 8) MQ_QUANTIZE(8);
-    else MQ_QUANTIZE(16);
+  if (K % V == 0 && stride % V == 0 && aligned16(x) && (reinterpret_cast<uintptr_t>(q) & 7u) == 0 && nvec <= 256 * 8) {
+#define MQ_QUANTIZE(NV, TPR) \
+  quantize_rows<T, NV, TPR><<<(unsigned)((rows + 256 / TPR - 1) / (256 / TPR)), 256, 0, st>>>(xs, stride, rows, (int)K, q, scale)
+    if (nvec <= 32) MQ_QUANTIZE(1, 32);
+    else if (nvec <= 32 * 2) MQ_QUANTIZE(2, 32);
+    else if (nvec <= 32 * 3) MQ_QUANTIZE(3, 32);
+    else if (nvec <= 32 * 4) MQ_QUANTIZE(4, 32);
+    else if (nvec <= 256) MQ_QUANTIZE(1, 256);
+    else if (nvec <= 256 * 2) MQ_QUANTIZE(2, 256);
+    else if (nvec <= 256 * 4) MQ_QUANTIZE(4, 256);
+    else MQ_QUANTIZE(8, 256);
 #undef MQ_QUANTIZE
   } else {
     quantize_any_rows<T><<<(unsigned)rows, 256, 0, st>>>(xs, stride, K, q, scale);
