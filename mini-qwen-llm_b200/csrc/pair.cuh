@@ -24,6 +24,10 @@ __device__ __forceinline__ uint32_t in_leader(uint32_t addr) {
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// The same without waiting for this thread's own loads and stores: for what was only read, and has arrived.
+__device__ __forceinline__ void arrive_cluster_relaxed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 // Bounded wait of a warp on a barrier that the other CTA signals too.
 __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* d_status) {
   uint32_t ok;

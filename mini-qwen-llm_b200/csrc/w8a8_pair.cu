@@ -418,117 +418,160 @@ w8a8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     const uint32_t stg_s = smem_addr(stg);
     const int mi = lane >> 3, ri = lane & 7;
     auto place = [&](int tok, int piece) { return (uint32_t)(tok * ROWB + ((piece ^ ((tok * PIECES >> 3) & (PIECES - 1))) << 4)); };
+    // two tokens' sums times their scales, times the channel's (as w8_value, two at a time)
+    auto scaled = [](uint32_t lo, uint32_t hi, f32x2 rows, float channel) {
+      return unpack2(mul2(mul2(pack2(__int2float_rn((int)lo), __int2float_rn((int)hi)), rows), pack2(channel, channel)));
+    };
     OutT* out = reinterpret_cast<OutT*>(A.out);
-    uint32_t used = 0;
-    int cur = 0;
-    bool ok = true;
-    for (int nth = 0; deal(nth) < total && ok; ++nth) {
-      const W8Tile w = table.locate(deal(nth));
-      const int b0 = w.two ? 0 : cur;
+    // An accumulator's share of a tile: its token rows, this warp's columns, and the scales the lane needs.
+    struct Chunk {
+      int row0, nrow, col0;                        // first token row and token rows; first output column of the warp
+      float ws[2][2];                              // of the lane's weight rows: [half][row, row + 8]; SwiGLU: half 0 gate, half 1 up
+      float xs[4];                                 // of the token that the lane stands for in each block
+    };
+    auto chunk_of = [&](const W8Tile& w, int c) {
+      Chunk k;
+      const bool second_rows = c == 1 && w.shape == TOKENS2;
+      k.row0 = w.tok0 + (second_rows ? w.n0 : 0);
+      k.nrow = second_rows ? w.ntok - w.n0 : min(w.ntok, w.n0);
+      k.col0 = (w.unit + (c == 1 && w.shape == WEIGHTS2 ? 1 : 0)) * 2 * CW + rank * CW + quad * (CW / 4);
       const float* ws = A.w_scale + (size_t)(w.expert % A.period) * (SWIGLU ? 2 * N : N);
-      for (int c = 0; c < (w.two ? 2 : 1); ++c) {
-        const int b = c == 0 ? b0 : 1;
-        const bool second_rows = c == 1 && w.shape == TOKENS2;
-        const int row0 = w.tok0 + (second_rows ? w.n0 : 0);                // first token row of the accumulator
-        const int nrow = second_rows ? w.ntok - w.n0 : min(w.ntok, w.n0);
-        const int col0 = (w.unit + (c == 1 && w.shape == WEIGHTS2 ? 1 : 0)) * 2 * CW + rank * CW + quad * (CW / 4);
-        // scales of the lane's weight rows: [half][row, row + 8]; SwiGLU: half 0 gate, half 1 up
-        float wsc[2][2];
 #pragma unroll
-        for (int hl = 0; hl < 2; ++hl)
+      for (int hl = 0; hl < 2; ++hl)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int col = col0 + (SWIGLU ? 0 : 16 * hl) + 8 * j + (lane >> 2);
-            wsc[hl][j] = col < N ? ws[SWIGLU && hl == 1 ? N + col : col] : 0.0f;
-          }
-        const int rounds = max(0, (nrow - 32 * group + 63) >> 6);
-        float xsc[4];                                                      // of the token that the lane stands for in each block
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 32 * group + 64 * i + lane;
-          xsc[i] = r < nrow ? A.x_scale[w8_source(A, row0 + r)] : 0.0f;
+        for (int j = 0; j < 2; ++j) {
+          const int col = k.col0 + (SWIGLU ? 0 : 16 * hl) + 8 * j + (lane >> 2);
+          k.ws[hl][j] = col < N ? ws[SWIGLU && hl == 1 ? N + col : col] : 0.0f;
         }
-        ok = mbar_wait_warp(tfull(b), (used >> b) & 1u, abort_flag, d_status);
-        if (!ok) break;
-        used ^= 1u << b;
-        fence_after_sync();
-        // Blocks leave tensor memory (packed) ahead of their stores, so that the accumulator is free early and the stores run
-        // under the next tile's MMAs: all four, or two at a time where registers are short.
-        constexpr int PACKED = SWIGLU ? 8 : 16;
-        constexpr int BATCH = sizeof(OutT) == 4 ? 1 : GATHER && !SWIGLU ? 2 : 4;
 #pragma unroll
-        for (int i0 = 0; i0 < 4; i0 += BATCH) {
-          uint32_t v[BATCH][PACKED];
+      for (int i = 0; i < 4; ++i) {
+        const int r = 32 * group + 64 * i + lane;
+        k.xs[i] = r < k.nrow ? A.x_scale[w8_source(A, k.row0 + r)] : 0.0f;
+      }
+      return k;
+    };
+    uint32_t used = 0;
+    int cur = 0, nth = 0, c = 0;
+    bool ok = true;
+    W8Tile w;
+    Chunk k;
+    if (deal(0) < total) {
+      w = table.locate(deal(0));
+      k = chunk_of(w, 0);
+    }
+    while (deal(nth) < total) {
+      const int b = c == 1 ? 1 : w.two ? 0 : cur;
+      // the next chunk's scales come from afar (its rows through the permutation): they travel while this one is finished
+      const bool same = c == 0 && w.two;
+      W8Tile next = w;
+      if (!same && deal(nth + 1) < total) next = table.locate(deal(nth + 1));
+      Chunk ahead = k;
+      if (same || deal(nth + 1) < total) ahead = chunk_of(next, same ? 1 : 0);
+      ok = mbar_wait_warp(tfull(b), (used >> b) & 1u, abort_flag, d_status);
+      if (!ok) break;
+      used ^= 1u << b;
+      fence_after_sync();
+      const int blocks = max(0, (k.nrow - 32 * group + 63) >> 6);          // of 32 tokens, every other one
+      constexpr int PACKED = SWIGLU ? 8 : 16;
+      // Blocks leave tensor memory two at a time.  The accumulator is free once the last two are in registers, and what follows
+      // runs under the next tile's MMAs.
+      auto load = [&](int i0, uint32_t (&f)[2][2][16]) {
 #pragma unroll
-          for (int i = 0; i < BATCH; ++i) {
-            if (i0 + i < rounds) {
-              uint32_t f[2][16];
-              const uint32_t ta = tmem + b * WN + ((uint32_t)(quad * 32) << 16) + 32 * group + 64 * (i0 + i);
-              tmem_ld_frag(ta, f[0]);
-              tmem_ld_frag(ta + (16u << 16), f[1]);
-              tmem_ld_wait();
+        for (int i = 0; i < 2; ++i) {
+          if (i0 + i < blocks) {
+            const uint32_t ta = tmem + b * WN + ((uint32_t)(quad * 32) << 16) + 32 * group + 64 * (i0 + i);
+            tmem_ld_frag(ta, f[i][0]);
+            tmem_ld_frag(ta + (16u << 16), f[i][1]);
+          }
+        }
+        tmem_ld_wait();
+      };
+      auto release = [&] {
+        fence_before_sync();
+        __syncwarp();
+        // relaxed: the sums are in registers, and a release would wait for the stores of the chunk before and the loads for the
+        // next (half of the finishing warps' time)
+        if (lane == 0) arrive_cluster_relaxed(in_leader(tempty(b)));
+      };
+      auto scale = [&](int i0, const uint32_t (&f)[2][2][16], uint32_t (&v)[2][PACKED]) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {                                // token octets
-                const float s0 = __shfl_sync(0xffffffffu, xsc[i0 + i], 8 * j + 2 * (lane & 3));
-                const float s1 = __shfl_sync(0xffffffffu, xsc[i0 + i], 8 * j + 2 * (lane & 3) + 1);
+        for (int i = 0; i < 2; ++i) {
+          if (i0 + i < blocks) {
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {                              // weight rows lane / 4 and lane / 4 + 8
-                  float a0 = w8_value((int)f[0][4 * j + 2 * q], s0, wsc[0][q]);
-                  float a1 = w8_value((int)f[0][4 * j + 2 * q + 1], s1, wsc[0][q]);
-                  float c0 = w8_value((int)f[1][4 * j + 2 * q], s0, wsc[1][q]);
-                  float c1 = w8_value((int)f[1][4 * j + 2 * q + 1], s1, wsc[1][q]);
-                  if (SWIGLU) {
-                    a0 = w8_swiglu(a0, c0);
-                    a1 = w8_swiglu(a1, c1);
-                  }
-                  if (sizeof(OutT) == 4) {
-                    const int r = 32 * group + 64 * (i0 + i) + 8 * j + 2 * (lane & 3), col = col0 + 8 * q + (lane >> 2);
-                    float* o = reinterpret_cast<float*>(out) + (size_t)(row0 + r) * N + col;
-                    if (r < nrow && col < N) o[0] = a0;
-                    if (r + 1 < nrow && col < N) o[N] = a1;
-                    if (!SWIGLU && r < nrow && col + 16 < N) o[16] = c0;
-                    if (!SWIGLU && r + 1 < nrow && col + 16 < N) o[N + 16] = c1;
-                  } else {
-                    v[i][2 * j + q] = pack16<OutT>(a0, a1);
-                    if (!SWIGLU) v[i][(8 + 2 * j + q) % PACKED] = pack16<OutT>(c0, c1);
-                  }
+            for (int j = 0; j < 4; ++j) {                                  // token octets
+              const f32x2 s01 = pack2(__shfl_sync(0xffffffffu, k.xs[i0 + i], 8 * j + 2 * (lane & 3)),
+                                      __shfl_sync(0xffffffffu, k.xs[i0 + i], 8 * j + 2 * (lane & 3) + 1));
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {                                // weight rows lane / 4 and lane / 4 + 8
+                const float2 x = scaled(f[i][0][4 * j + 2 * q], f[i][0][4 * j + 2 * q + 1], s01, k.ws[0][q]);
+                const float2 y = scaled(f[i][1][4 * j + 2 * q], f[i][1][4 * j + 2 * q + 1], s01, k.ws[1][q]);
+                const float a0 = SWIGLU ? w8_swiglu(x.x, y.x) : x.x, a1 = SWIGLU ? w8_swiglu(x.y, y.y) : x.y;
+                if (sizeof(OutT) == 4) {
+                  const int r = 32 * group + 64 * (i0 + i) + 8 * j + 2 * (lane & 3), col = k.col0 + 8 * q + (lane >> 2);
+                  float* o = reinterpret_cast<float*>(out) + (size_t)(k.row0 + r) * N + col;
+                  if (r < k.nrow && col < N) o[0] = a0;
+                  if (r + 1 < k.nrow && col < N) o[N] = a1;
+                  if (!SWIGLU && r < k.nrow && col + 16 < N) o[16] = y.x;
+                  if (!SWIGLU && r + 1 < k.nrow && col + 16 < N) o[N + 16] = y.y;
+                } else {
+                  v[i][2 * j + q] = pack16<OutT>(a0, a1);
+                  if (!SWIGLU) v[i][(8 + 2 * j + q) % PACKED] = pack16<OutT>(y.x, y.y);
                 }
               }
             }
           }
-          if (i0 + BATCH == 4) {
-            fence_before_sync();
+        }
+      };
+      auto store = [&](int i0, const uint32_t (&v)[2][PACKED]) {
+        if (sizeof(OutT) == 4) return;                                     // stored from the fragments
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (i0 + i < blocks) {
+            const int r = 32 * group + 64 * (i0 + i);
+            __syncwarp();                                                  // the previous block's rows have been read
+#pragma unroll
+            for (int j2 = 0; j2 < 2; ++j2) {                               // token octets (0, 1) and (2, 3)
+              const int tok = 8 * (2 * j2 + (mi >> 1)) + ri;
+#pragma unroll
+              for (int hl = 0; hl < (SWIGLU ? 1 : 2); ++hl)
+                stmatrix_x4_trans(stg_s + place(tok, 2 * hl + (mi & 1)), v[i][(8 * hl + 4 * j2) % PACKED],
+                                  v[i][(8 * hl + 4 * j2 + 1) % PACKED], v[i][(8 * hl + 4 * j2 + 2) % PACKED],
+                                  v[i][(8 * hl + 4 * j2 + 3) % PACKED]);
+            }
             __syncwarp();
-            if (lane == 0) arrive_cluster(in_leader(tempty(b)));
-          }
-          if (sizeof(OutT) == 4) continue;
 #pragma unroll
-          for (int i = 0; i < BATCH; ++i) {
-            if (i0 + i < rounds) {
-              const int r = 32 * group + 64 * (i0 + i);
-              __syncwarp();                                                // the previous block's rows have been read
-#pragma unroll
-              for (int j2 = 0; j2 < 2; ++j2) {                             // token octets (0, 1) and (2, 3)
-                const int tok = 8 * (2 * j2 + (mi >> 1)) + ri;
-#pragma unroll
-                for (int hl = 0; hl < (SWIGLU ? 1 : 2); ++hl)
-                  stmatrix_x4_trans(stg_s + place(tok, 2 * hl + (mi & 1)), v[i][(8 * hl + 4 * j2) % PACKED],
-                                    v[i][(8 * hl + 4 * j2 + 1) % PACKED], v[i][(8 * hl + 4 * j2 + 2) % PACKED],
-                                    v[i][(8 * hl + 4 * j2 + 3) % PACKED]);
-              }
-              __syncwarp();
-#pragma unroll
-              for (int q = 0; q < PIECES; ++q) {
-                const int row = (32 / PIECES) * q + lane / PIECES, p = lane % PIECES;
-                if (row < nrow - r && col0 + p * 8 < N)
-                  *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + (size_t)(row0 + r + row) * N + col0 + p * 8) =
-                      *reinterpret_cast<const uint4*>(stg + place(row, p));
-              }
+            for (int q = 0; q < PIECES; ++q) {
+              const int row = (32 / PIECES) * q + lane / PIECES, p = lane % PIECES;
+              if (row < k.nrow - r && k.col0 + p * 8 < N)
+                *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + (size_t)(k.row0 + r + row) * N + k.col0 + p * 8) =
+                    *reinterpret_cast<const uint4*>(stg + place(row, p));
             }
           }
         }
+      };
+      uint32_t f[2][2][16], v[2][PACKED];
+      load(0, f);
+      if (blocks > 2) {
+        scale(0, f, v);
+        load(2, f);
+        release();
+        store(0, v);
+        scale(2, f, v);
+        store(2, v);
+      } else {
+        release();
+        scale(0, f, v);
+        store(0, v);
       }
-      cur = w.two ? 0 : cur ^ 1;
+      if (same) {
+        c = 1;
+      } else {
+        cur = w.two ? 0 : cur ^ 1;
+        c = 0;
+        ++nth;
+        w = next;
+      }
+      k = ahead;
     }
   }
 

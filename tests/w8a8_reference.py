@@ -41,5 +41,8 @@ def assert_close(out, ref, extra=0.0):
 
 def swiglu_extra(g):
     """A relative error d of g moves silu(g) by at most (1 + |g|) d; g and u carry three roundings each (u's are in
-    assert_close already), exp two units in the last place, the sum, the quotient and the product one rounding each."""
-    return (1 + g) * 3 * 2.0 ** -24 + 6 * 2.0 ** -23
+    assert_close already): 3 (1 + |g|) 2^-24.  The exponential's argument |g| log2(e) is rounded once and its constant is off by
+    half a step, 1.5 * 2^-24 relative, which the exponential turns into 1.5 |g| 2^-24 (together below 5 (1 + |g|) 2^-24).  The
+    exponential itself is 2^-22 off, the sum 2^-24, the reciprocal 2^-23 and the three products 2^-24 each: 10 * 2^-24, below
+    6 * 2^-23."""
+    return (1 + g) * 5 * 2.0 ** -24 + 6 * 2.0 ** -23
