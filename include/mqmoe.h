@@ -389,6 +389,22 @@ int mq_w8a8_grouped_swiglu(const int8_t* x, const float* x_scale, const int32_t*
                            const int8_t* w_gate_up, const float* w_scale, const int32_t* offsets, int64_t S, int64_t E,
                            int64_t weight_period, int64_t I, int64_t H, int out_dtype, void* h, int32_t* d_status,
                            void* stream);
+/* The same products from rows of floating-point numbers (x_dtype, row_stride elements apart), quantised by the call: what a
+ * program calls that has no other use for the int8 rows.
+ * mq_w8a8_linear_x: up to 16 rows of at most 16384 elements in all (Kd a multiple of 16) take one launch and no workspace, more
+ *   take two.  mq_w8a8_grouped_x: mq_w8a8_grouped_gemm, or with swiglu != 0 mq_w8a8_grouped_swiglu (perm as there, else NULL);
+ *   offsets of 32 or 64 bits; zero_uncovered != 0 writes zeros to the rows of out that no group covers.
+ * workspace: mq_w8a8_workspace_bytes(rows of x, Kd, groups) bytes, 16-byte aligned, overwritten.  h_launches (optional) receives
+ * the number of kernels launched. */
+size_t mq_w8a8_workspace_bytes(int64_t rows, int64_t Kd, int64_t groups);
+int mq_w8a8_linear_x(const void* x, int x_dtype, int64_t row_stride, const int8_t* qweight, const float* w_scale, int64_t M,
+                     int64_t N, int64_t Kd, int out_dtype, void* workspace, size_t workspace_bytes, void* out,
+                     int32_t* d_status, int32_t* h_launches, void* stream);
+int mq_w8a8_grouped_x(const void* x, int x_dtype, int64_t row_stride, const int32_t* perm, int64_t T, int64_t top_k,
+                      const int8_t* qweight, const float* w_scale, const void* offsets, int offsets_are_64, int64_t S, int64_t E,
+                      int64_t weight_period, int64_t N, int64_t Kd, int swiglu, int zero_uncovered, int out_dtype,
+                      void* workspace, size_t workspace_bytes, void* out, int32_t* d_status, int32_t* h_launches,
+                      void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * The whole block in one call: what Qwen3MoEBlock.forward (mini_qwen/model/layers/moe.py:49-68) computes on one

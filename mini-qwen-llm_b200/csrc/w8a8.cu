@@ -14,6 +14,11 @@ namespace mq {
 bool w8a8_pair_covers(const W8Args& A, bool swiglu);
 int w8a8_pair(const W8Args& A, bool swiglu, int out_dtype, int32_t* d_status, cudaStream_t st);
 
+// A few rows of floating-point numbers, quantised in the same launch (w8a8_rows.cu).
+bool w8a8_rows_covers(const void* x, int x_dtype, int64_t stride, const void* w, int64_t M, int64_t N, int64_t K);
+int w8a8_rows(const void* x, int x_dtype, int64_t stride, const int8_t* w, const float* w_scale, int64_t M, int64_t N, int64_t K,
+              int out_dtype, void* out, cudaStream_t st);
+
 namespace {
 
 constexpr int G_M = 64, G_N = 64, G_K = 64;        // rows, columns and bytes of k of a tile
@@ -133,6 +138,12 @@ int w8a8_dispatch(W8Args A, bool swiglu, int out_dtype, int32_t* d_status, cudaS
   if (A.S == 0) return MQ_OK;
   if (A.T == 0 || !A.x || !A.x_scale || !A.w || !A.w_scale || !A.out) return MQ_ERR_INVALID_ARGUMENT;
   if (A.perm == nullptr && A.T < A.S) return MQ_ERR_INVALID_ARGUMENT;
+  if (A.top_k > 1) {                               // m = ceil(2^(32 + s) / k) with 2^s >= k / 2 divides every n < 2^31 exactly
+    int shift = 0;
+    while ((2ull << shift) < (unsigned long long)A.top_k) ++shift;
+    A.k_mul = (uint32_t)(((1ull << (32 + shift)) + A.top_k - 1) / A.top_k);
+    A.k_shift = (uint32_t)shift;
+  }
   if (w8a8_pair_covers(A, swiglu)) return w8a8_pair(A, swiglu, out_dtype, d_status, st);
   A.words = ((A.K | (int)(reinterpret_cast<uintptr_t>(A.x) & 3u) | (int)(reinterpret_cast<uintptr_t>(A.w) & 3u)) & 3) == 0;
   if (out_dtype == MQ_F32) return launch_generic<float>(A, swiglu, st);
@@ -156,7 +167,7 @@ extern "C" int mq_w8a8_grouped_gemm(const int8_t* x, const float* x_scale, const
   if (S > 0 && !offsets) return MQ_ERR_INVALID_ARGUMENT;
   if (!sizes_fit(S, S, E, 1, N, Kd)) return MQ_ERR_UNSUPPORTED_SHAPE;
   return w8a8_dispatch(W8Args{x, x_scale, qweight, w_scale, offsets, nullptr, (int)S, (int)S, 1, (int)E, (int)weight_period,
-                              (int)N, (int)Kd, 0, out},
+                              (int)N, (int)Kd, out, 0, 0, 0},
                        false, out_dtype, d_status, reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -164,7 +175,7 @@ extern "C" int mq_w8a8_linear(const int8_t* x, const float* x_scale, const int8_
                               int64_t N, int64_t Kd, int out_dtype, void* out, int32_t* d_status, void* stream) {
   using namespace mq;
   if (!sizes_fit(M, M, 1, 1, N, Kd)) return MQ_ERR_UNSUPPORTED_SHAPE;
-  return w8a8_dispatch(W8Args{x, x_scale, qweight, w_scale, nullptr, nullptr, (int)M, (int)M, 1, 1, 1, (int)N, (int)Kd, 0, out},
+  return w8a8_dispatch(W8Args{x, x_scale, qweight, w_scale, nullptr, nullptr, (int)M, (int)M, 1, 1, 1, (int)N, (int)Kd, out, 0, 0, 0},
                        false, out_dtype, d_status, reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -176,6 +187,85 @@ extern "C" int mq_w8a8_grouped_swiglu(const int8_t* x, const float* x_scale, con
   if (S > 0 && !offsets) return MQ_ERR_INVALID_ARGUMENT;
   if (!sizes_fit(S, T, E, top_k, I, H)) return MQ_ERR_UNSUPPORTED_SHAPE;
   return w8a8_dispatch(W8Args{x, x_scale, w_gate_up, w_scale, offsets, perm, (int)S, (int)T, (int)top_k, (int)E,
-                              (int)weight_period, (int)I, (int)H, 0, h},
+                              (int)weight_period, (int)I, (int)H, h, 0, 0, 0},
                        true, out_dtype, d_status, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t mq_w8a8_workspace_bytes(int64_t rows, int64_t Kd, int64_t groups) {
+  if (rows < 0 || Kd < 0 || groups < 0) return 256;
+  auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+  return up((size_t)(rows * Kd)) + up((size_t)rows * 4) + up((size_t)(groups + 1) * 4);
+}
+
+namespace {
+struct W8Space {                                   // a workspace cut up
+  int8_t* q;
+  float* scale;
+  int32_t* offsets;
+  W8Space(void* p, int64_t rows, int64_t Kd) {
+    auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    uint8_t* b = reinterpret_cast<uint8_t*>(p);
+    q = reinterpret_cast<int8_t*>(b);
+    scale = reinterpret_cast<float*>(b + up((size_t)(rows * Kd)));
+    offsets = reinterpret_cast<int32_t*>(b + up((size_t)(rows * Kd)) + up((size_t)rows * 4));
+  }
+};
+}  // namespace
+
+extern "C" int mq_w8a8_linear_x(const void* x, int x_dtype, int64_t row_stride, const int8_t* qweight, const float* w_scale,
+                                int64_t M, int64_t N, int64_t Kd, int out_dtype, void* workspace, size_t workspace_bytes,
+                                void* out, int32_t* d_status, int32_t* h_launches, void* stream) {
+  using namespace mq;
+  if (h_launches) *h_launches = 0;
+  if (M < 0 || N <= 0 || Kd <= 0 || row_stride < 0 || !valid_dtype(x_dtype) || !valid_dtype(out_dtype))
+    return MQ_ERR_INVALID_ARGUMENT;
+  if (!sizes_fit(M, M, 1, 1, N, Kd)) return MQ_ERR_UNSUPPORTED_SHAPE;
+  if (M == 0) return MQ_OK;
+  if (!x || !qweight || !w_scale || !out) return MQ_ERR_INVALID_ARGUMENT;
+  if (w8a8_rows_covers(x, x_dtype, row_stride, qweight, M, N, Kd)) {
+    if (h_launches) *h_launches = 1;
+    return w8a8_rows(x, x_dtype, row_stride, qweight, w_scale, M, N, Kd, out_dtype, out, reinterpret_cast<cudaStream_t>(stream));
+  }
+  if (!workspace || !aligned16(workspace)) return MQ_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < mq_w8a8_workspace_bytes(M, Kd, 0)) return MQ_ERR_WORKSPACE_TOO_SMALL;
+  const W8Space ws(workspace, M, Kd);
+  const int rc = mq_quantize_rows_int8(x, x_dtype, M, Kd, row_stride, ws.q, ws.scale, stream);
+  if (rc != MQ_OK) return rc;
+  if (h_launches) *h_launches = 2;
+  return mq_w8a8_linear(ws.q, ws.scale, qweight, w_scale, M, N, Kd, out_dtype, out, d_status, stream);
+}
+
+extern "C" int mq_w8a8_grouped_x(const void* x, int x_dtype, int64_t row_stride, const int32_t* perm, int64_t T, int64_t top_k,
+                                 const int8_t* qweight, const float* w_scale, const void* offsets, int offsets_are_64, int64_t S,
+                                 int64_t E, int64_t weight_period, int64_t N, int64_t Kd, int swiglu, int zero_uncovered,
+                                 int out_dtype, void* workspace, size_t workspace_bytes, void* out, int32_t* d_status,
+                                 int32_t* h_launches, void* stream) {
+  using namespace mq;
+  if (h_launches) *h_launches = 0;
+  if (S < 0 || T < 0 || E <= 0 || N <= 0 || Kd <= 0 || row_stride < 0 || !valid_dtype(x_dtype) || !valid_dtype(out_dtype) ||
+      weight_period <= 0 || weight_period > E || top_k <= 0 || (perm != nullptr && !swiglu))
+    return MQ_ERR_INVALID_ARGUMENT;
+  if (!sizes_fit(S, T, E, top_k, N, Kd)) return MQ_ERR_UNSUPPORTED_SHAPE;
+  if (S == 0) return MQ_OK;
+  if (T == 0 || !x || !qweight || !w_scale || !offsets || !out || !workspace || !aligned16(workspace) ||
+      (perm == nullptr && T < S))
+    return MQ_ERR_INVALID_ARGUMENT;
+  if (workspace_bytes < mq_w8a8_workspace_bytes(T, Kd, E)) return MQ_ERR_WORKSPACE_TOO_SMALL;
+  const W8Space ws(workspace, T, Kd);
+  int n = 2;
+  const int32_t* off = reinterpret_cast<const int32_t*>(offsets);
+  if (offsets_are_64 || zero_uncovered) {
+    const int rc = mq_grouped_prepare(offsets, offsets_are_64, S, E, N, out_dtype, zero_uncovered ? out : nullptr,
+                                      offsets_are_64 ? ws.offsets : nullptr, nullptr, stream);
+    if (rc != MQ_OK) return rc;
+    if (offsets_are_64) off = ws.offsets;
+    ++n;
+  }
+  int rc = mq_quantize_rows_int8(x, x_dtype, T, Kd, row_stride, ws.q, ws.scale, stream);
+  if (rc != MQ_OK) return rc;
+  if (h_launches) *h_launches = n;
+  if (swiglu)
+    return mq_w8a8_grouped_swiglu(ws.q, ws.scale, perm, T, top_k, qweight, w_scale, off, S, E, weight_period, N, Kd, out_dtype,
+                                  out, d_status, stream);
+  return mq_w8a8_grouped_gemm(ws.q, ws.scale, qweight, w_scale, off, S, E, weight_period, N, Kd, out_dtype, out, d_status, stream);
 }

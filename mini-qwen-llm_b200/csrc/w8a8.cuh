@@ -14,14 +14,17 @@ struct W8Args {
   const int32_t* perm;         // row r of the sorted order is row perm[r] / top_k of x; null: row r
   int S, T, top_k, E, period;
   int N, K;                    // N: output columns (SwiGLU: gate rows, then as many up rows)
-  int words;                   // rows of x and w start at multiples of four bytes
   void* out;                   // [S, N]
+  int words;                   // rows of x and w start at multiples of four bytes
+  uint32_t k_mul, k_shift;     // n / top_k = umulhi(n, k_mul) >> k_shift for n < 2^31; k_mul 0: n
 };
 
 // Offsets outside 0..S, and permutation entries outside x, are the caller's mistake; they must not become addresses.
 __device__ __forceinline__ int w8_offset(const W8Args& A, int e) { return min(max(A.offsets[e], 0), A.S); }
 __device__ __forceinline__ size_t w8_source(const W8Args& A, int row) {
-  return A.perm == nullptr ? (size_t)row : (size_t)min(max(A.perm[row], 0) / A.top_k, A.T - 1);
+  if (A.perm == nullptr) return (size_t)row;
+  const uint32_t slot = (uint32_t)max(A.perm[row], 0);
+  return min(A.k_mul == 0 ? slot : __umulhi(slot, A.k_mul) >> A.k_shift, (uint32_t)(A.T - 1));
 }
 
 // The sum may pass 2^24, so the conversion rounds; with the two products that is 1.5 * 2^-23 in all at most.
@@ -31,8 +34,7 @@ __device__ __forceinline__ float w8_value(int sum, float row_scale, float channe
 // silu(g) * u with the hardware's exponential and reciprocal: 2^-22 and 2^-23 relative, and the exponent's rounding makes
 // 1.5 |g| 2^-24, all far below the rounding of a 16-bit result.  With the exponential of -|g| nothing overflows and the
 // denominator is in 1..2; where it is below 2^-126 (g < -87) the result is 0, off by less than 1e-36 |u|.  The library's expf
-// and a true quotient took 40 instructions more, and the finishing warps were what the gate/up product waited for (4096 tokens
-// on 128 experts: W8_SWIGLU_BEFORE against W8_SWIGLU_AFTER us).
+// and a true quotient take some 40 instructions more for each of the 25 million outputs of 4096 tokens (132 against 125 us).
 __device__ __forceinline__ float w8_swiglu(float g, float u) {
   float p, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(__fmul_rn(fabsf(g), -1.44269504f)));

@@ -73,6 +73,7 @@ struct W8Tile {
 // Tiles are dealt out in the groups' order, the pairs in turn; with skewed groups and more than one round of tiles, largest
 // groups first and the pairs back and forth (a tile of 512 rows takes four times one of 128).
 struct W8Table {
+  __device__ static int weight_of(const W8Args& A, int expert) { return A.period == A.E ? expert : expert % A.period; }
   const int* off;                                // [E + 1]
   const int* group;                              // [E]: the groups by size, or null: in their own order
   const int* first;                              // [E + 1]: first tile of the group in that order
@@ -101,8 +102,9 @@ struct W8Table {
       w.n0 = (n + 31) & ~31;
       return w;
     }
-    const int cuts = (n + most - 1) / most, cut = local / units;
-    const int width = (((n + cuts - 1) / cuts) + 31) & ~31;                // balanced
+    // balanced cuts; mostly there is one, and no division to wait for
+    const int cuts = n <= most ? 1 : (n + most - 1) / most, cut = cuts == 1 ? 0 : local / units;
+    const int width = ((cuts == 1 ? n : (n + cuts - 1) / cuts) + 31) & ~31;
     w.unit = local - cut * units;
     w.tok0 = off[e] + cut * width;
     w.ntok = max(0, min(width, n - cut * width));
@@ -241,7 +243,7 @@ w8a8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     };
     for (int nth = 0; deal(nth) < total && ok; ++nth) {
       const W8Tile w = table.locate(deal(nth));
-      const int we = (int)uniform(w.expert % A.period), unit = (int)uniform(w.unit), shape = (int)uniform(w.shape);
+      const int we = (int)uniform(W8Table::weight_of(A, w.expert)), unit = (int)uniform(w.unit), shape = (int)uniform(w.shape);
       const bool two = uniform(w.two) != 0;
       const int h0 = (int)uniform(w.n0 >> 1), h1 = (int)uniform(w.n1 >> 1);     // this CTA's halves of the token chunks
       const int box0 = (h0 + W_BOX - 1) / W_BOX, box1 = (h1 + W_BOX - 1) / W_BOX;   // rows past the half: not read
@@ -435,7 +437,7 @@ w8a8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
       k.row0 = w.tok0 + (second_rows ? w.n0 : 0);
       k.nrow = second_rows ? w.ntok - w.n0 : min(w.ntok, w.n0);
       k.col0 = (w.unit + (c == 1 && w.shape == WEIGHTS2 ? 1 : 0)) * 2 * CW + rank * CW + quad * (CW / 4);
-      const float* ws = A.w_scale + (size_t)(w.expert % A.period) * (SWIGLU ? 2 * N : N);
+      const float* ws = A.w_scale + (size_t)W8Table::weight_of(A, w.expert) * (SWIGLU ? 2 * N : N);
 #pragma unroll
       for (int hl = 0; hl < 2; ++hl)
 #pragma unroll

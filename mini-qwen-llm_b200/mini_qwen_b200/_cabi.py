@@ -57,6 +57,9 @@ PROTOTYPES = {
     "mq_w8a8_grouped_gemm": (c_int, [_P, _P, _P, _P, _P, _L, _L, _L, _L, _L, _I, _P, _P, _P]),
     "mq_w8a8_linear": (c_int, [_P, _P, _P, _P, _L, _L, _L, _I, _P, _P, _P]),
     "mq_w8a8_grouped_swiglu": (c_int, [_P, _P, _P, _L, _L, _P, _P, _P, _L, _L, _L, _L, _L, _I, _P, _P, _P]),
+    "mq_w8a8_workspace_bytes": (c_size_t, [_L, _L, _L]),
+    "mq_w8a8_linear_x": (c_int, [_P, _I, _L, _P, _P, _L, _L, _L, _I, _P, c_size_t, _P, _P, _P, _P]),
+    "mq_w8a8_grouped_x": (c_int, [_P, _I, _L, _P, _L, _L, _P, _P, _P, _I, _L, _L, _L, _L, _L, _I, _I, _I, _P, c_size_t, _P, _P, _P, _P]),
     "mq_moe_forward_workspace_bytes": (c_size_t, [_P, _L]),
     "mq_moe_forward": (c_int, [_P, _P, _P, c_float, _P, _L, _P, c_size_t, _P, c_size_t, _P, _P, _P, _P]),
     "mq_moe_small_covers": (c_int, [_P, _L]),
@@ -143,31 +146,27 @@ def require_cuda(*tensors: torch.Tensor) -> None:
             raise ValueError("these kernels run on CUDA tensors only; there is no CPU path")
 
 
-def one_device(*tensors: torch.Tensor | None) -> torch.device:
-    """The device that all of a call's tensors lie on."""
-    require_cuda(*tensors)
-    device = tensors[0].device
+def one_device(*tensors: torch.Tensor | None) -> int:
+    """The index of the device that all of a call's tensors (the first is not None) lie on."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"the tensors of a call lie on one device; got {device} and {t.device}")
-    return device
+        if t is not None and t.get_device() != index:
+            require_cuda(*tensors)
+            raise ValueError(f"the tensors of a call lie on one device; got {tensors[0].device} and {t.device}")
+    if index < 0:
+        require_cuda(*tensors)
+    return index
 
 
-class current_device:
-    """Launches inside go to ``device``, whichever is the current one (a no-op where it already is)."""
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
-    def __init__(self, device: torch.device):
-        self._index, self._before = device.index, None
 
-    def __enter__(self):
-        now = torch.cuda.current_device()
-        if self._index is not None and self._index != now:
-            torch.cuda.set_device(self._index)
-            self._before = now
-
-    def __exit__(self, *exc):
-        if self._before is not None:
-            torch.cuda.set_device(self._before)
+def on_device(index: int, fn, *args):
+    """``fn(*args)`` with device ``index`` (that of a tensor, so CUDA is initialised) the current one."""
+    if _current_device() == index:
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
 
 
 def check(status: int, what: str) -> None:

@@ -29,7 +29,7 @@ def _layer(x, router_weight, inter, top_k, bias, renormalize, group_size=0, int8
                           router=router_weight.data_ptr(), router_bias=None if bias is None else bias.data_ptr())
 
 
-def _call(layer: _cabi.MoELayer, x, residual, status, device) -> torch.Tensor:
+def _call(layer: _cabi.MoELayer, x, residual, status, index) -> torch.Tensor:
     H = layer.hidden
     if x.shape[-1:] != (H,):
         raise ValueError(f"x must be [..., {H}], got {tuple(x.shape)}")
@@ -51,12 +51,12 @@ def _call(layer: _cabi.MoELayer, x, residual, status, device) -> torch.Tensor:
     if not lib.mq_moe_small_covers(address, T):
         raise ValueError(f"{T} tokens of this layer (hidden {H}, inter {layer.inter}, {layer.experts} experts, top_k {layer.top_k}) "
                          "are outside what the two-launch layer covers")
-    with _cabi.current_device(device):
-        space = lib.mq_moe_small_workspace_bytes(address, T)
-        ws = torch.empty(space, dtype=torch.uint8, device=device)
-        rc = lib.mq_moe_small(address, rows.data_ptr(), _cabi.ptr(residual), T, ws.data_ptr(), space, out.data_ptr(),
-                              _cabi.ptr(status), _cabi.stream_ptr(device))
-    _cabi.check(rc, "mq_moe_small")
+    space = lib.mq_moe_small_workspace_bytes(address, T)
+    ws = torch.empty(space, dtype=torch.uint8, device=x.device)
+    rc = _cabi.on_device(index, lib.mq_moe_small, address, rows.data_ptr(), _cabi.ptr(residual), T, ws.data_ptr(), space,
+                         out.data_ptr(), _cabi.ptr(status), _cabi.stream_ptr(index))
+    if rc:
+        _cabi.check(rc, "mq_moe_small")
     _cabi.count_launches(2)
     return out
 
@@ -82,7 +82,7 @@ def moe_layer_small(hidden_states: torch.Tensor, router_weight: torch.Tensor, ga
     The ``top_k`` experts with the largest logits (``+ bias``, fp32 [E]; equal ones by ascending id) are weighted by their softmax
     scores, divided by their sum with ``renormalize``.  ``residual`` is added before the one rounding.  ``status`` (int32 [1],
     optional) receives device-side error bits (a bounded wait that ran out)."""
-    device = _cabi.one_device(hidden_states, router_weight, gate_up_weights, down_weights, bias, residual, status)
+    index = _cabi.one_device(hidden_states, router_weight, gate_up_weights, down_weights, bias, residual, status)
     router_weight = _router(hidden_states, router_weight)
     E, H = router_weight.shape
     if gate_up_weights.dim() != 3 or gate_up_weights.shape[0] != E or gate_up_weights.shape[1] % 2 or gate_up_weights.shape[2] != H:
@@ -95,7 +95,7 @@ def moe_layer_small(hidden_states: torch.Tensor, router_weight: torch.Tensor, ga
     _aligned(gate_up_weights, down_weights)
     layer = _layer(hidden_states, router_weight, I, top_k, bias, renormalize)
     layer.gate[0], layer.down[0] = gate_up_weights.data_ptr(), down_weights.data_ptr()
-    return _call(layer, hidden_states, residual, status, device)
+    return _call(layer, hidden_states, residual, status, index)
 
 
 def w4a16_moe_layer_small(hidden_states: torch.Tensor, router_weight: torch.Tensor, gate, up, down, top_k: int = 8,
@@ -103,7 +103,7 @@ def w4a16_moe_layer_small(hidden_states: torch.Tensor, router_weight: torch.Tens
                           residual: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`moe_layer_small` on int4 experts: ``gate``, ``up`` and ``down`` are ``(qweight [E, K/8, N], scales [E, K/g, N],
     qzeros [E, K/g, N/8])`` stacks as in :func:`w4a16_grouped_gemm`; bf16, group sizes that are multiples of 128."""
-    device = _cabi.one_device(hidden_states, router_weight, *gate, *up, *down, bias, residual, status)
+    index = _cabi.one_device(hidden_states, router_weight, *gate, *up, *down, bias, residual, status)
     router_weight = _router(hidden_states, router_weight)
     E, H = router_weight.shape
     if hidden_states.dtype != torch.bfloat16:
@@ -122,7 +122,7 @@ def w4a16_moe_layer_small(hidden_states: torch.Tensor, router_weight: torch.Tens
     for field, trio in ((layer.gate, gate), (layer.up, up), (layer.down, down)):
         for i, t in enumerate(trio):
             field[i] = t.data_ptr()
-    return _call(layer, hidden_states, residual, status, device)
+    return _call(layer, hidden_states, residual, status, index)
 
 
 def w8a8_moe_layer_small(hidden_states: torch.Tensor, router_weight: torch.Tensor, gate_up, down, top_k: int = 8,
@@ -131,7 +131,7 @@ def w8a8_moe_layer_small(hidden_states: torch.Tensor, router_weight: torch.Tenso
     """:func:`moe_layer_small` on int8 experts: ``gate_up`` is (int8 [E, 2I, H], scales fp32 [E, 2I]), ``down`` (int8 [E, H, I],
     scales fp32 [E, H]).  The token rows and the rows of h are quantised to int8 as :func:`quantize_rows_int8` does; bf16, fp16
     or fp32 activations."""
-    device = _cabi.one_device(hidden_states, router_weight, *gate_up, *down, bias, residual, status)
+    index = _cabi.one_device(hidden_states, router_weight, *gate_up, *down, bias, residual, status)
     router_weight = _router(hidden_states, router_weight)
     E, H = router_weight.shape
     w13, s13 = gate_up
@@ -148,4 +148,4 @@ def w8a8_moe_layer_small(hidden_states: torch.Tensor, router_weight: torch.Tenso
     layer = _layer(hidden_states, router_weight, I, top_k, bias, renormalize, int8=True)
     layer.gate[0], layer.gate[1] = w13.data_ptr(), s13.data_ptr()
     layer.down[0], layer.down[1] = w2.data_ptr(), s2.data_ptr()
-    return _call(layer, hidden_states, residual, status, device)
+    return _call(layer, hidden_states, residual, status, index)

@@ -110,6 +110,29 @@ def test_linear(dtype, M, K, N):
     assert torch.equal(out, same)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N", [(1, 16, 1), (2, 512, 48), (3, 272, 17), (4, 4096, 100), (7, 2064, 31), (8, 4096, 33),
+                                   (9, 2048, 272), (16, 2048, 1000), (16, 16, 16), (1, 32768, 20), (13, 2512, 5)])
+def test_linear_of_a_few_rows(dtype, M, K, N):
+    """One launch that quantises the rows itself: the same numbers as from rows quantised before."""
+    g = gen(M * K + N)
+    x = hidden(g, M, K + 16, dtype=dtype)[:, :K]                 # rows that lie apart
+    w, s = weight(g, N, K)
+    out = w8a8_gemm(x, w, s)
+    q, sx = R.quantize(x)
+    R.assert_close(out, R.product(q, sx, w, s))
+    assert torch.equal(out, w8a8_gemm(q.to(torch.int8), w, s, x_scale=sx.float(), out_dtype=dtype))
+    for out_dtype in DTYPES:
+        R.assert_close(w8a8_gemm(x, w, s, out_dtype=out_dtype), R.product(q, sx, w, s))
+    x = x.clone()
+    x[M // 2, K // 3] = float("nan")
+    x[0, K - 1] = float("inf")
+    bad = w8a8_gemm(x, w, s)
+    assert torch.isnan(bad[M // 2]).all() and torch.isnan(bad[0]).all()
+    keep = [m for m in range(M) if m not in (0, M // 2)]
+    assert torch.equal(bad[keep], out[keep])
+
+
 @pytest.mark.parametrize("M", [1, 40, 300])
 def test_linear_sums_are_exact_at_the_largest_magnitudes(M):
     """All products 128 * 128: the int32 sum reaches 2^31 - 2^14 at the longest K."""
