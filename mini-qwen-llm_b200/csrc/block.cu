@@ -22,13 +22,14 @@ namespace {
 
 // How a call runs.
 struct BlockPlan {
-  bool w4, small, prepared, tile, stream, tc5, gather_in_kernel;
+  bool w4, w8, small, prepared, tile, stream, tc5, gather_in_kernel;
 };
 
 BlockPlan plan_of(const mq_moe_layer& L, int64_t T) {
   const int64_t H = L.hidden, I = L.inter, E = L.experts, K = L.top_k, S = T * K;
   BlockPlan p = {};
   p.w4 = L.group_size > 0;
+  p.w8 = L.int8_experts != 0;
   // decode batches: logits, top-k, plan (and the W4A16 activation preparation) in one launch
   p.small = T <= 64 && E <= 256 && K <= 32 && S <= 2048;
   if (p.w4) {
@@ -41,6 +42,8 @@ BlockPlan plan_of(const mq_moe_layer& L, int64_t T) {
     p.stream = !p.tile && streams;
     p.prepared = !p.tile && prepared;
     p.gather_in_kernel = p.tile || p.stream;
+  } else if (p.w8) {
+    p.gather_in_kernel = true;
   } else {
     p.tc5 = L.dtype == MQ_BF16 && tc5_covers(S, E, I, H, true) && T * H < ((int64_t)1 << 32);
     p.gather_in_kernel = p.tc5 || generic_small_groups(S, E, I, true);
@@ -60,6 +63,8 @@ struct BlockSpace {
 };
 struct BlockBuffers {
   void *xn, *rows, *h, *y, *xp;
+  int8_t *xq, *hq;
+  float *xq_scale, *hq_scale;
   float *xs, *weights, *logits;
   int32_t *ids32, *perm, *inv, *offsets;
   void* plan_ws;
@@ -89,6 +94,12 @@ size_t carve(const mq_moe_layer& L, int64_t T, const BlockPlan& p, bool norm, ui
     b.xs = (float*)s.take((size_t)n * 32 * 4);
   }
   if (!p.gather_in_kernel) b.rows = s.take((size_t)(S * H) * el);
+  if (p.w8) {
+    b.xq = (int8_t*)s.take((size_t)(T * H));
+    b.xq_scale = (float*)s.take((size_t)T * 4);
+    b.hq = (int8_t*)s.take((size_t)(S * I));
+    b.hq_scale = (float*)s.take((size_t)S * 4);
+  }
   b.h = s.take((size_t)(S * I) * el);
   b.y = s.take((size_t)(S * H) * el);
   return s.used;
@@ -96,7 +107,8 @@ size_t carve(const mq_moe_layer& L, int64_t T, const BlockPlan& p, bool norm, ui
 
 bool layer_ok(const mq_moe_layer* L) {
   return L != nullptr && L->hidden > 0 && L->inter > 0 && L->experts > 0 && L->top_k > 0 && L->group_size >= 0 &&
-         valid_dtype(L->dtype) && valid_dtype(L->router_dtype) && !L->int8_experts && (L->group_size == 0 || L->dtype == MQ_BF16);
+         valid_dtype(L->dtype) && valid_dtype(L->router_dtype) && !(L->int8_experts && L->group_size > 0) &&
+         (L->group_size == 0 || L->dtype == MQ_BF16);
 }
 
 }  // namespace
@@ -153,7 +165,16 @@ extern "C" int mq_moe_forward(const mq_moe_layer* h_layer, const void* x, const 
     MQ_BLOCK_STEP(mq_gather_rows(x, L.dtype, b.perm, S, K, H, b.rows, stream));
     ++n;
   }
-  if (!p.w4) {
+  if (p.w8) {
+    const int8_t *w13 = reinterpret_cast<const int8_t*>(L.gate[0]), *w2 = reinterpret_cast<const int8_t*>(L.down[0]);
+    const float *s13 = reinterpret_cast<const float*>(L.gate[1]), *s2 = reinterpret_cast<const float*>(L.down[1]);
+    MQ_BLOCK_STEP(mq_quantize_rows_int8(x, L.dtype, T, H, H, b.xq, b.xq_scale, stream));
+    MQ_BLOCK_STEP(mq_w8a8_grouped_swiglu(b.xq, b.xq_scale, b.perm, T, K, w13, s13, b.offsets, S, E, E, I, H, L.dtype, b.h, d_status,
+                                         stream));
+    MQ_BLOCK_STEP(mq_quantize_rows_int8(b.h, L.dtype, S, I, I, b.hq, b.hq_scale, stream));
+    MQ_BLOCK_STEP(mq_w8a8_grouped_gemm(b.hq, b.hq_scale, w2, s2, b.offsets, S, E, E, H, I, L.dtype, b.y, d_status, stream));
+    n += 2;
+  } else if (!p.w4) {
     if (p.tc5)
       MQ_BLOCK_STEP(mq_grouped_swiglu_gather(x, b.perm, L.gate[0], b.offsets, T, K, E, E, I, H, L.dtype, b.h, d_status, stream));
     else if (p.gather_in_kernel)

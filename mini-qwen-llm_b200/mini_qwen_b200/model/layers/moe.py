@@ -30,8 +30,11 @@ from ...kernels.w4a16_gemm import (w4a16_grouped_gemm, w4a16_grouped_swiglu,
                                      w4a16_tc_swiglu)
 from ... import parallel
 from .linear_w4a16 import LinearW4A16
+from .linear_w8a8 import LinearW8A8
+from ...kernels.w8a8_gemm import w8a8_grouped_gemm, w8a8_grouped_swiglu_gather
 
 _PROJ = ("gate_proj", "up_proj", "down_proj")
+_QUANTISED = (LinearW4A16, LinearW8A8)
 
 
 class _ExpertMLP(nn.Module):
@@ -74,6 +77,17 @@ class _NativeLayer:
         self.launches = ctypes.c_int32(0)
         self.launches_address = ctypes.addressof(self.launches)
         self._bytes: dict = {}
+        self._small: dict = {}
+        # the two-launch layer reads 16 bytes of a weight at a time
+        self.aligned = all((p or 0) % 16 == 0 for p in (layer.gate[0], layer.up[0], layer.down[0]))
+
+    def small_workspace_bytes(self, lib, T: int) -> int:
+        """Workspace of the two-launch layer, 0 where it does not cover the call."""
+        n = self._small.get(T)
+        if n is None:
+            covered = self.aligned and lib.mq_moe_small_covers(self.address, T)
+            n = self._small[T] = lib.mq_moe_small_workspace_bytes(self.address, T) if covered else 0
+        return n
 
     def workspace_bytes(self, lib, T: int) -> int:
         n = self._bytes.get(T)
@@ -130,6 +144,9 @@ class Qwen3MoEBlock(nn.Module):
         # the fp32 logit sums
         self.fuse_small_batches = True
         self.fuse_max_tokens = 64
+        # up to 16 tokens: the whole layer in two launches (one rounding, at the end, instead of one after every operation).
+        # None: where the experts are W8A8; True: wherever the call is covered; False: nowhere
+        self.small_layer = None
         # expert-parallel W4A16 decode batches (at most 64 tokens over all ranks): "replicate" = every rank holds
         # all tokens and runs its own experts (two rank barriers per call), "dispatch" = the prefill path
         self.ep_decode = "replicate"
@@ -160,22 +177,34 @@ class Qwen3MoEBlock(nn.Module):
             experts = self._modules["experts"]._modules
             first = experts["0"]._modules["gate_proj"]
             last = experts[str(self.num_local_experts - 1)]._modules["down_proj"]
-            a = first._buffers["qweight"] if isinstance(first, LinearW4A16) else first._parameters["weight"]
-            b = last._buffers["qweight"] if isinstance(last, LinearW4A16) else last._parameters["weight"]
+            a = first._buffers["qweight"] if isinstance(first, _QUANTISED) else first._parameters["weight"]
+            b = last._buffers["qweight"] if isinstance(last, _QUANTISED) else last._parameters["weight"]
         except KeyError:        # not kept there: parametrizations, weight norm, wrapped modules, replicas
             first, last = self.experts[0].gate_proj, self.experts[-1].down_proj
-            a = first.qweight if isinstance(first, LinearW4A16) else first.weight
-            b = last.qweight if isinstance(last, LinearW4A16) else last.weight
+            a = first.qweight if isinstance(first, _QUANTISED) else first.weight
+            b = last.qweight if isinstance(last, _QUANTISED) else last.weight
         return (a.data_ptr(), b.data_ptr())
 
     def finalize(self) -> None:
         """Gather the per-expert tensors into expert-major stacks (idempotent)."""
-        kinds = {isinstance(getattr(ex, p), LinearW4A16) for ex in self.experts for p in _PROJ}
+        kinds = {next((q for q in _QUANTISED if isinstance(getattr(ex, p), q)), None) for ex in self.experts for p in _PROJ}
         if len(kinds) != 1:
-            raise ValueError("experts mix nn.Linear and LinearW4A16 projections; quantise all or none")
-        quantised = kinds.pop()
+            raise ValueError("experts mix nn.Linear, LinearW4A16 and LinearW8A8 projections; quantise all one way or none")
+        kind = kinds.pop()
         with torch.no_grad():
-            if quantised:
+            if kind is LinearW8A8:
+                stacks = {"w4": False, "w8": True}
+                gate, up, down = ([getattr(ex, p) for ex in self.experts] for p in _PROJ)
+                inter = gate[0].out_features
+                for key, buf in (("w13", "qweight"), ("s13", "scales")):
+                    stacks[key] = torch.stack([torch.cat([getattr(g, buf), getattr(u, buf)]) for g, u in zip(gate, up)])
+                    for e, (g, u) in enumerate(zip(gate, up)):
+                        g._buffers[buf], u._buffers[buf] = stacks[key][e, :inter], stacks[key][e, inter:]
+                for key, buf in (("w2", "qweight"), ("s2", "scales")):
+                    stacks[key] = torch.stack([getattr(d, buf) for d in down])
+                    for e, d in enumerate(down):
+                        d._buffers[buf] = stacks[key][e]
+            elif kind is LinearW4A16:
                 stacks = {"w4": True}
                 groups = {getattr(ex, p).group_size for ex in self.experts for p in _PROJ}
                 if len(groups) != 1:
@@ -270,6 +299,33 @@ class Qwen3MoEBlock(nn.Module):
         blk._stacked_sentinel = blk._sentinel()
         return blk
 
+    @classmethod
+    def from_stacked_w8(cls, config, router_weight: torch.Tensor, gate_up, down) -> "Qwen3MoEBlock":
+        """Builds a W8A8 block from expert-major stacks without copying them: ``gate_up`` is (int8 [E, 2I, H], scales fp32
+        [E, 2I]), gate rows first, ``down`` (int8 [E, H, I], scales fp32 [E, H]), as ``quantize_channels_int8`` gives them.
+        The per-expert ``LinearW8A8`` modules become views of the stacks."""
+        with torch.device("meta"):
+            blk = cls(config)
+        E, H, I = blk.num_experts, config.hidden_size, config.intermediate_size
+        (w13, s13), (w2, s2) = ((w.contiguous(), s.contiguous()) for w, s in (gate_up, down))
+        for what, w, c, shape in (("gate_up", w13, s13, (E, 2 * I, H)), ("down", w2, s2, (E, H, I))):
+            if tuple(w.shape) != shape or tuple(c.shape) != shape[:2] or w.dtype != torch.int8 or c.dtype != torch.float32:
+                raise ValueError(f"{what} must be int8 {list(shape)} with float32 scales {list(shape[:2])}")
+        if tuple(router_weight.shape) != (E, H):
+            raise ValueError(f"router_weight must be [{E}, {H}], got {tuple(router_weight.shape)}")
+        blk.gate.weight = nn.Parameter(router_weight, requires_grad=False)
+        for e, ex in enumerate(blk.experts):
+            for name, w, s in (("gate_proj", w13[e, :I], s13[e, :I]), ("up_proj", w13[e, I:], s13[e, I:]),
+                               ("down_proj", w2[e], s2[e])):
+                with torch.device("meta"):
+                    lin = LinearW8A8(w.shape[1], w.shape[0])
+                lin._buffers["qweight"], lin._buffers["scales"] = w, s
+                setattr(ex, name, lin)
+        blk._stacks = {"w4": False, "w8": True, "w13": w13, "s13": s13, "w2": w2, "s2": s2}
+        blk._stacked_epoch = blk._epoch[0]
+        blk._stacked_sentinel = blk._sentinel()
+        return blk
+
     def _ready(self):
         if (self._stacks is None or self._stacked_epoch != self._epoch[0]
                 or self._stacked_sentinel != self._sentinel()):
@@ -285,7 +341,7 @@ class Qwen3MoEBlock(nn.Module):
         out = self._forward_native(x, residual, None, 0.0)
         return out if out is not None else self._forward_staged(x, residual)
 
-    def _native_layer(self):
+    def _native_layer(self, dtype=None):
         """The layer's description for :func:`mq_moe_forward`, made again when anything it points to has changed; None
         when the whole-block call does not apply (expert parallelism, stage timing, a kernel chosen by hand, a router
         weight that its module computes: the description holds addresses, the module has to hold the tensor)."""
@@ -300,6 +356,10 @@ class Qwen3MoEBlock(nn.Module):
         # the layouts beside the addresses: another view of the same storage, or a tensor at a freed one's place
         key = (self._stacked_epoch, self._stacked_sentinel, _layout(router), None if bias is None else _layout(bias),
                self.norm_topk_prob, self.num_experts_per_tok)
+        w8 = st.get("w8", False)
+        if w8:                        # its weights go with activations of any type
+            dtype = router.dtype if dtype is None else dtype
+            key += (dtype,)
         native = self._native
         if native is not None and native[0] == key:
             return native[1]
@@ -308,7 +368,7 @@ class Qwen3MoEBlock(nn.Module):
         dense = not st["w4"]
         w = st["w13"] if dense else st["gate_proj"][0]
         if (router.is_cuda and router.is_contiguous() and w.is_cuda and w.get_device() == router.get_device()
-                and router.dtype in _cabi._DTYPES and (not dense or w.dtype in _cabi._DTYPES)
+                and router.dtype in _cabi._DTYPES and (not dense or (dtype if w8 else w.dtype) in _cabi._DTYPES)
                 and E == self.num_experts and self.num_experts_per_tok <= 32
                 and (bias is None or (bias.dtype == torch.float32 and bias.is_contiguous() and bias.is_cuda
                                       and bias.numel() == E))):
@@ -316,24 +376,28 @@ class Qwen3MoEBlock(nn.Module):
                                router_dtype=_cabi.dtype_code(router), router=router.data_ptr(),
                                router_bias=None if bias is None else bias.data_ptr())
             if dense:
-                L.inter, L.group_size, L.dtype = w.shape[1] // 2, 0, _cabi.dtype_code(w)
+                L.inter, L.group_size, L.dtype = w.shape[1] // 2, 0, _cabi._DTYPES[dtype] if w8 else _cabi.dtype_code(w)
                 L.gate[0], L.down[0] = w.data_ptr(), st["w2"].data_ptr()
+                if w8:
+                    L.int8_experts, L.gate[1], L.down[1] = 1, st["s13"].data_ptr(), st["s2"].data_ptr()
             else:
                 L.inter, L.group_size, L.dtype = w.shape[2], st["group_size"], _cabi.MQ_BF16
                 for name in ("gate", "up", "down"):
                     for i, t in enumerate(st[name + "_proj"]):
                         getattr(L, name)[i] = t.data_ptr()
-            made = _NativeLayer(L, w.dtype if dense else torch.bfloat16, w.get_device(), H)
+            made = _NativeLayer(L, dtype if w8 else w.dtype if dense else torch.bfloat16, w.get_device(), H)
         self._native = (key, made)
         return made
 
     def _forward_native(self, x, residual, norm_weight, norm_eps: float):
         """The whole block in one library call, or None when it does not apply to these tensors."""
-        nat = self._native_layer()
+        nat = self._native_layer(x.dtype)
         if nat is None or x.dtype != nat.dtype or x.get_device() != nat.device or x.shape[-1] != nat.hidden:
             return None
         if not x.is_contiguous():
             x = x.contiguous()
+        if x.data_ptr() % 16:                        # a view into a larger buffer: the kernels read 16 bytes at a time
+            x = x.clone()
         T = x.numel() // nat.hidden
         if T == 0:
             return None
@@ -343,6 +407,12 @@ class Qwen3MoEBlock(nn.Module):
             if not residual.is_contiguous():
                 residual = residual.contiguous()
         out = torch.empty_like(x)
+        small = self.small_layer
+        if T <= 16 and (nat.layer.int8_experts if small is None else small):
+            lib = _cabi.load()
+            space = nat.small_workspace_bytes(lib, T)
+            if space:
+                return self._forward_small(nat, lib, x, residual, norm_weight, norm_eps, T, space, out)
         route_ws = None
         if T <= 64:
             route_ws = self._route_ws
@@ -354,14 +424,34 @@ class Qwen3MoEBlock(nn.Module):
         lib = _cabi.load()
         space = nat.workspace_bytes(lib, T)
         ws = torch.empty(space, dtype=torch.uint8, device=x.device)
-        rc = lib.mq_moe_forward(nat.address, x.data_ptr(), norm_weight, norm_eps,
-                                None if residual is None else residual.data_ptr(), T,
-                                None if route_ws is None else route_ws.data_ptr(), 0 if route_ws is None else route_ws.numel(),
-                                ws.data_ptr(), space, out.data_ptr(), status.data_ptr(), nat.launches_address,
-                                _cabi.stream_ptr(nat.device))
+        rc = _cabi.on_device(nat.device, lib.mq_moe_forward, nat.address, x.data_ptr(), norm_weight, norm_eps,
+                             None if residual is None else residual.data_ptr(), T,
+                             None if route_ws is None else route_ws.data_ptr(), 0 if route_ws is None else route_ws.numel(),
+                             ws.data_ptr(), space, out.data_ptr(), status.data_ptr(), nat.launches_address,
+                             _cabi.stream_ptr(nat.device))
         if rc:
             _cabi.check(rc, "mq_moe_forward")
         _cabi.count_launches(nat.launches.value)
+        return out
+
+    def _forward_small(self, nat, lib, x, residual, norm_weight, norm_eps: float, T: int, space: int, out):
+        """A few tokens: the layer in two launches (three with the norm)."""
+        stream = _cabi.stream_ptr(nat.device)
+        if norm_weight is not None:
+            rows = torch.empty_like(x)
+            rc = _cabi.on_device(nat.device, lib.mq_rms_norm, x.data_ptr(), nat.layer.dtype, norm_weight, norm_eps, T, nat.hidden,
+                                 rows.data_ptr(), stream)
+            if rc:
+                _cabi.check(rc, "mq_rms_norm")
+            x = rows
+        ws = torch.empty(space, dtype=torch.uint8, device=x.device)
+        status = self._status_word(x.device)
+        rc = _cabi.on_device(nat.device, lib.mq_moe_small, nat.address, x.data_ptr(),
+                             None if residual is None else residual.data_ptr(), T, ws.data_ptr(), space, out.data_ptr(),
+                             status.data_ptr(), stream)
+        if rc:
+            _cabi.check(rc, "mq_moe_small")
+        _cabi.count_launches(2 if norm_weight is None else 3)
         return out
 
     def _forward_staged(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
@@ -376,6 +466,8 @@ class Qwen3MoEBlock(nn.Module):
             res = residual.reshape(-1, shape[-1]).contiguous()
         K, E = self.num_experts_per_tok, self.num_experts
         st = self._ready()
+        if st.get("w8") and self.ep_size > 1:
+            raise ValueError("W8A8 experts do not run expert-parallel")
 
         run = self._stage
         xp_tok = xs_tok = None
@@ -398,6 +490,11 @@ class Qwen3MoEBlock(nn.Module):
             perm, inv, off32, _ = run("permute_plan", moe_permute_plan, ids32, E, want_int64_offsets=False)
         if self.ep_size > 1 and self.ep_mode == "p2p":
             return self._forward_peer(x2d, st, weights, ids32, perm, inv, off32, T, K, E, res).reshape(shape)
+        if st.get("w8"):
+            status = self._status_word(x2d.device)
+            h = run("grouped_swiglu", w8a8_grouped_swiglu_gather, x2d, perm, K, st["w13"], st["s13"], off32, status=status)
+            out_perm = run("grouped_down", w8a8_grouped_gemm, h, st["w2"], st["s2"], off32, zero_init=False, status=status)
+            return run("unpermute_combine", unpermute_combine, out_perm, weights, inv, T, K, residual=res).reshape(shape)
         if self.ep_size == 1 and not st["w4"] and gather_swiglu_supported(x2d, st["w13"]):
             # the gate/up kernel fetches the rows through the permutation itself: no permuted copy
             status = self._status_word(x2d.device)
@@ -633,3 +730,14 @@ class Qwen3MoEBlock(nn.Module):
         for expert in self.experts:
             for p in _PROJ:
                 setattr(expert, p, LinearW4A16.from_float(getattr(expert, p), group_size).to(device))
+
+    def quantize_to_w8a8(self) -> None:
+        """Replace every expert Linear by an int8 ``LinearW8A8`` (a scale for each output channel) on the same device; the
+        activations are quantised as they come, token by token.  The router stays as it is."""
+        if self.ep_size > 1:
+            raise ValueError("W8A8 experts do not run expert-parallel")
+        if not all(isinstance(getattr(ex, p), nn.Linear) for ex in self.experts for p in _PROJ):
+            raise ValueError("quantize_to_w8a8 starts from nn.Linear projections")
+        for expert in self.experts:
+            for p in _PROJ:
+                setattr(expert, p, LinearW8A8.from_float(getattr(expert, p)))

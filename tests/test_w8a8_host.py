@@ -4,7 +4,8 @@ import torch
 
 from mini_qwen_b200 import _cabi
 from mini_qwen_b200.kernels import quantize_rows_int8, w8a8_gemm, w8a8_grouped_gemm, w8a8_grouped_swiglu
-from mini_qwen_b200.model.layers import LinearW8A8
+from mini_qwen_b200 import Qwen3MoEConfig
+from mini_qwen_b200.model.layers import LinearW8A8, Qwen3MoEBlock
 from mini_qwen_b200.quantization import quantize_channels_int8
 import w8a8_reference as R
 
@@ -72,3 +73,37 @@ def test_c_calls_check_their_arguments():
     assert lib.mq_w8a8_grouped_swiglu(one, one, None, 3, 1, one, one, one, 4, 2, 2, 8, 16, 1, one, None, None) == 1
     assert lib.mq_w8a8_grouped_swiglu(one, one, one, 0, 1, one, one, one, 4, 2, 2, 8, 16, 1, one, None, None) == 1
     assert lib.mq_w8a8_grouped_swiglu(one, one, one, 3, 0, one, one, one, 4, 2, 2, 8, 16, 1, one, None, None) == 1
+
+
+def _block(**kw):
+    cfg = Qwen3MoEConfig(hidden_size=64, intermediate_size=32, num_experts=4, num_experts_per_tok=2)
+    return cfg, Qwen3MoEBlock(cfg, **kw)
+
+
+def test_block_swaps_its_projections_for_int8_ones():
+    cfg, blk = _block()
+    want = quantize_channels_int8(blk.experts[2].up_proj.weight.data)
+    blk.quantize_to_w8a8()
+    lin = blk.experts[2].up_proj
+    assert isinstance(lin, LinearW8A8) and torch.equal(lin.qweight, want[0]) and torch.equal(lin.scales, want[1])
+    blk.finalize()
+    assert blk._stacks["w13"].shape == (4, 64, 64) and blk._stacks["s13"].shape == (4, 64)
+    assert torch.equal(blk._stacks["w13"][2, 32:], want[0]) and torch.equal(blk._stacks["s13"][2, 32:], want[1])
+    other = Qwen3MoEBlock.from_stacked_w8(cfg, blk.gate.weight.data, (blk._stacks["w13"], blk._stacks["s13"]),
+                                          (blk._stacks["w2"], blk._stacks["s2"]))
+    a, b = blk.state_dict(), other.state_dict()
+    assert a.keys() == b.keys() and all(torch.equal(a[k], b[k]) for k in a)
+    with pytest.raises(ValueError):
+        blk.quantize_to_w8a8()                      # quantised already
+
+
+def test_block_refuses_mixed_experts_and_wrong_stacks():
+    cfg, blk = _block()
+    blk.experts[1].down_proj = LinearW8A8.from_float(blk.experts[1].down_proj)
+    with pytest.raises(ValueError):
+        blk.finalize()
+    q = torch.zeros(4, 64, 64, dtype=torch.int8), torch.zeros(4, 64)
+    d = torch.zeros(4, 64, 32, dtype=torch.int8), torch.zeros(4, 64)
+    for bad in ((q, (d[0], d[1][:, :32])), ((q[0][:3], q[1]), d), ((q[0].float(), q[1]), d)):
+        with pytest.raises(ValueError):
+            Qwen3MoEBlock.from_stacked_w8(cfg, blk.gate.weight.data, *bad)
