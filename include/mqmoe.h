@@ -414,7 +414,7 @@ int mq_w8a8_grouped_x(const void* x, int x_dtype, int64_t row_stride, const int3
  *   dense layers (group_size 0, any dtype): gate[0] = w13 [E, 2*inter, hidden] (gate rows, then up rows),
  *     down[0] = w2 [E, hidden, inter];
  *   W4A16 layers (dtype MQ_BF16): gate / up / down = {qweight, scales, qzeros} of the stacks;
- *   W8A8 layers (int8_experts != 0, group_size 0; dtype: that of x and out): gate = {w13 int8 [E, 2*inter, hidden],
+ *   W8A8 layers (int8_experts == 1, group_size 0; dtype: that of x and out): gate = {w13 int8 [E, 2*inter, hidden],
  *     scales fp32 [E, 2*inter]}, down = {w2 int8 [E, hidden, inter], scales fp32 [E, hidden]}; x and
  *     the rows of h are quantised as mq_quantize_rows_int8 does, h = silu(g) * u rounded once before.
  * route_workspace: as mq_route_small's (zero-filled once by the caller, for 64 tokens, kept between calls that are

@@ -29,7 +29,7 @@ BlockPlan plan_of(const mq_moe_layer& L, int64_t T) {
   const int64_t H = L.hidden, I = L.inter, E = L.experts, K = L.top_k, S = T * K;
   BlockPlan p = {};
   p.w4 = L.group_size > 0;
-  p.w8 = L.int8_experts != 0;
+  p.w8 = L.int8_experts == 1;
   // decode batches: logits, top-k, plan (and the W4A16 activation preparation) in one launch
   p.small = T <= 64 && E <= 256 && K <= 32 && S <= 2048;
   if (p.w4) {
@@ -107,7 +107,7 @@ size_t carve(const mq_moe_layer& L, int64_t T, const BlockPlan& p, bool norm, ui
 
 bool layer_ok(const mq_moe_layer* L) {
   return L != nullptr && L->hidden > 0 && L->inter > 0 && L->experts > 0 && L->top_k > 0 && L->group_size >= 0 &&
-         valid_dtype(L->dtype) && valid_dtype(L->router_dtype) && !(L->int8_experts && L->group_size > 0) &&
+         valid_dtype(L->dtype) && valid_dtype(L->router_dtype) && !(L->int8_experts == 1 && L->group_size > 0) &&
          (L->group_size == 0 || L->dtype == MQ_BF16);
 }
 

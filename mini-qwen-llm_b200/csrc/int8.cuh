@@ -37,9 +37,12 @@ static __device__ __noinline__ int exact_quotient(float x, float scale) {
   return (int)fmin(fmax(rint(__ddiv_rn((double)x, (double)scale)), -127.0), 127.0);
 }
 
-// N values to bytes.  1.5 * 2^23 + x * inv, rounded once, has the nearest whole number in its low bits.  x * inv is off the
-// quotient by |q| 2^-24 < 8e-6 at most, so the number is the right one unless x * inv lies within 1.6e-5 of a half; there
-// the quotient is taken exactly.  No clamp: |x| * inv <= 127 (1 + 2^-22).
+// N values to bytes.  1.5 * 2^23 + x * inv, rounded once, has the nearest whole number n in its low bits.  x * inv is off the
+// quotient by |q| 2^-24 < 8e-6 at most, so n is the right one unless x * inv lies within 1.6e-5 of a half h = n +- 1/2.  There
+// the sign of x - h * scale decides, which one fused multiply-add gives exactly (h * scale has 32 bits, and no difference
+// from 2^-120 on vanishes); 0 is a half, which goes to the even side.  16-bit numbers meet halves often: half of the row's
+// maximum is 63.5.  (With a quotient in 64 bits there, 32768 rows of 2048 bf16 numbers took 77 us.)  No clamp:
+// |x| * inv <= 127 (1 + 2^-22).
 template <int N>
 __device__ __forceinline__ void quantize(const float (&x)[N], const RowScale& r, uint32_t (&q)[N / 4]) {
   constexpr float MAGIC = 12582912.0f;
@@ -51,14 +54,15 @@ __device__ __forceinline__ void quantize(const float (&x)[N], const RowScale& r,
     y[i] = __float_as_uint(v);
     off = fmaxf(off, fabsf(__fmaf_rn(x[i], r.inv, __fsub_rn(MAGIC, v))));
   }
-  if (r.inv == 0.0f && !r.exact) {                               // zeros, or no numbers
+  if (r.inv == 0.0f) {                                           // zeros, no numbers, or tiny ones
 #pragma unroll
-    for (int i = 0; i < N; ++i) y[i] = 0u;
-  } else if (r.exact || off > 0.499984f) {
+    for (int i = 0; i < N; ++i) y[i] = r.exact ? (uint32_t)exact_quotient(x[i], r.scale) : 0u;
+  } else if (off > 0.499984f) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float d = r.exact ? 1.0f : fabsf(__fmaf_rn(x[i], r.inv, MAGIC - __uint_as_float(y[i])));
-      if (d > 0.499984f) y[i] = (uint32_t)exact_quotient(x[i], r.scale);
+      const float n = __fsub_rn(__uint_as_float(y[i]), MAGIC), d = __fmaf_rn(x[i], r.inv, -n), side = copysignf(1.0f, d);
+      const float past = side * __fmaf_rn(-__fmaf_rn(0.5f, side, n), r.scale, x[i]);
+      if (fabsf(d) > 0.499984f && (past > 0.0f || (past == 0.0f && (y[i] & 1u) != 0))) y[i] += d > 0.0f ? 1u : 0xffffffffu;
     }
   }
 #pragma unroll

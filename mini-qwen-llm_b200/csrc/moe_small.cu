@@ -1062,7 +1062,7 @@ __global__ void __launch_bounds__(Roles<F>::THREADS, 1) moe_small_layer(const Sm
 
 int format_of(const mq_moe_layer& L) {
   if (L.group_size > 0) return F_INT4;
-  if (L.int8_experts) return F_INT8;
+  if (L.int8_experts == 1) return F_INT8;
   return L.dtype == MQ_BF16 ? F_BF16 : F_F16;
 }
 
@@ -1099,7 +1099,7 @@ size_t carve_small(const mq_moe_layer& L, int64_t T, uint8_t* base, SmallArgs& A
 
 bool small_layer_ok(const mq_moe_layer* L) {
   return L != nullptr && L->hidden > 0 && L->inter > 0 && L->experts > 0 && L->top_k > 0 && L->group_size >= 0 &&
-         valid_dtype(L->dtype) && valid_dtype(L->router_dtype) && !(L->int8_experts && L->group_size > 0);
+         valid_dtype(L->dtype) && valid_dtype(L->router_dtype) && !(L->int8_experts == 1 && L->group_size > 0);
 }
 
 bool small_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank, const cuuint64_t* dims,
