@@ -308,3 +308,40 @@ def test_refusals():
     for call in bad:
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -110, 2.0 ** 100])
+def test_values_at_and_beside_every_half(dtype, size):
+    """The numbers nearest to (n + 1/2) * scale and their neighbours, for every n and many scales: the nearest whole number of
+    the exact quotient, halves to even."""
+    if dtype == torch.float16:
+        size = 1.0 if size < 1 else 2.0 ** 8
+    g = torch.Generator().manual_seed(11)
+    top = torch.cat([torch.tensor([1.0, 1.5, 127.0, 254.0 / 256, 1.0 + 2.0 ** -7]), 1 + torch.rand(59, generator=g)]) * size
+    top = top.to(dtype)
+    scale = R.quantize(top[:, None])[1].double()                                     # of a row that holds only its maximum
+    half = (torch.arange(-127, 127).double() + 0.5) * scale[:, None]
+    near = half.to(dtype)
+    bits = {4: torch.int32, 2: torch.int16}[near.element_size()]
+    beside = [(near.view(bits) + i).view(dtype) for i in (-2, -1, 0, 1, 2)]          # neighbours in magnitude
+    x = torch.cat([top[:, None], *beside], 1)
+    x = torch.where(x.abs() > top[:, None].abs(), top[:, None], x)
+    x = torch.cat([x, torch.zeros(x.shape[0], -x.shape[1] % 8, dtype=dtype)], 1)
+    rq, rs = R.quantize(x)
+    for data in (x, torch.cat([x, x], 1)[:, 1:x.shape[1] + 1]):                      # whole vectors, and rows off their grid
+        q, s = quantize_rows_int8(data.to(DEV))
+        want = rq if data is x else torch.cat([rq, rq], 1)[:, 1:x.shape[1] + 1]
+        assert torch.equal(s.cpu().double(), rs) and torch.equal(q.cpu().double(), want)
+
+
+@pytest.mark.parametrize("rows,cols", [(4096, 1032), (4097, 2048), (4099, 4096), (4101, 2056), (5001, 1024), (4098, 768)])
+def test_many_rows(rows, cols):
+    g = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, cols, generator=g).bfloat16()
+    x[rows - 1, 0] = float("nan")
+    x[rows // 2] = 0
+    q, s = quantize_rows_int8(x.to(DEV))
+    rq, rs = R.quantize(x)
+    assert torch.equal(q.cpu().double(), rq)
+    assert torch.equal(torch.nan_to_num(s.cpu().double(), nan=-1.0), torch.nan_to_num(rs, nan=-1.0))
