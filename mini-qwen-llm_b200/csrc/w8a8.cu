@@ -4,11 +4,12 @@
 // Follows the shapes of mini_qwen/kernels/moe_grouped_gemm.py:17-37 and mini_qwen/model/layers/moe.py:24-25; the
 // reference has no 8-bit path.  The int32 sums are exact (K <= 131071: 128 * 128 * K < 2^31).
 //
-// This file: the entry points, and the kernel for what the tensor-core kernel (w8a8_pair.cu) leaves: any size and alignment
-// (dot products of four bytes, tiles of 64 rows by 64 columns through shared memory).
+// This file: the entry points, and the kernel for what the CTA-pair kernel (w8a8_pair.cu) leaves: any size and alignment.
 #include "w8a8.cuh"
 
 namespace mq {
+
+int device_sm_count();
 
 // Tensor cores, CTA pairs (w8a8_pair.cu).
 bool w8a8_pair_covers(const W8Args& A, bool swiglu);
@@ -21,32 +22,64 @@ int w8a8_rows(const void* x, int x_dtype, int64_t stride, const int8_t* w, const
 
 namespace {
 
-constexpr int G_M = 64, G_N = 64, G_K = 64;        // rows, columns and bytes of k of a tile
-constexpr int G_LD = G_K / 4 + 1;                  // words of a staged row, padded
+constexpr int G_N = 64;                            // columns of a tile
 
-// Bytes [k, k + 4) of a row, zero past K.
-__device__ __forceinline__ int load_word(const int8_t* row, int k, int K, bool words) {
-  if (words && k + 4 <= K) return *reinterpret_cast<const int*>(row + k);
-  uint32_t w = 0;
+// 16 bytes [k, k + 16) of a row, zero past K: in one load where rows start at multiples of 16, else in words, put together
+// from their aligned neighbours where rows start anywhere.  Nothing outside [first, last), the tensor, is read.
+__device__ __forceinline__ int4 load_piece(const int8_t* row, int k, int K, int grid, const int8_t* first, const int8_t* last) {
+  const int8_t* p = row + k;
+  uint32_t w[4] = {};
+  if (k + 16 <= K) {
+    if (grid == 16) return *reinterpret_cast<const int4*>(p);
+    const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 3u;
+    if (off == 0) {
 #pragma unroll
-  for (int b = 0; b < 4; ++b)
-    if (k + b < K) w |= (uint32_t)(uint8_t)row[k + b] << (8 * b);
-  return (int)w;
+      for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+      return make_int4((int)w[0], (int)w[1], (int)w[2], (int)w[3]);
+    }
+    const int8_t* at = p - off;
+    if (at >= first && at + 20 <= last) {
+      uint32_t v[5];
+#pragma unroll
+      for (int i = 0; i < 5; ++i) v[i] = reinterpret_cast<const uint32_t*>(at)[i];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(v[i], v[i + 1], 8 * off);
+      return make_int4((int)w[0], (int)w[1], (int)w[2], (int)w[3]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (k + i < K) w[i >> 2] |= (uint32_t)(uint8_t)p[i] << (8 * (i & 3));
+  return make_int4((int)w[0], (int)w[1], (int)w[2], (int)w[3]);
 }
 
-template <typename OutT, bool SWIGLU>
+__device__ __forceinline__ void mma_s8(int (&c)[4], const int (&a)[4], int b0, int b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A tile of ROWS rows by 64 columns; blocks of KT bytes of k go through shared memory, the next one's pieces on their way in
+// registers.  64 rows: a warp has 16 rows and 32 columns; 16 rows: it has 8 columns.  What bounds it is the latency of a
+// block, about 2 us, so that few tiles take the larger blocks.  (Dot products of four bytes and single bytes off the grid, without
+// loads ahead: 1 row of K 777, N 333 33 us, now 8; 512 rows of K 1333, N 1499 89 us, now 28.)
+template <int ROWS, int KT, typename OutT, bool SWIGLU>
 __global__ void __launch_bounds__(256) w8a8_generic_kernel(const W8Args A) {
-  __shared__ int s_a[G_M * G_LD], s_b[(SWIGLU ? 2 : 1) * G_N * G_LD];
+  constexpr int SIDES = SWIGLU ? 2 : 1, LD = KT + 16, PIECES = KT / 16;                      // LD: no bank conflicts
+  constexpr int XP = ROWS * PIECES / 256, WP = SIDES * G_N * PIECES / 256;                   // pieces of a thread
+  constexpr int NT = ROWS == 64 ? 4 : 1;                                                     // 8-column tiles of a warp
+  static_assert(XP >= 1 && WP >= 1, "a piece for each thread");
+  __shared__ __align__(16) int8_t s_x[ROWS * LD];
+  __shared__ __align__(16) int8_t s_w[SIDES * G_N * LD];
   __shared__ int s_at[2];                          // group, first row of the tile
   const int tid = threadIdx.x;
   if (A.offsets == nullptr) {
-    if (tid == 0) { s_at[0] = 0; s_at[1] = (int)blockIdx.x * G_M; }
+    if (tid == 0) { s_at[0] = 0; s_at[1] = (int)blockIdx.x * ROWS; }
   } else if (tid < 32) {                           // the group that holds row tile blockIdx.x
     int before = 0, group = -1, first = 0;
     for (int e0 = 0; e0 < A.E && group < 0; e0 += 32) {
       const int e = e0 + tid;
       const int lo = e < A.E ? w8_offset(A, e) : 0, n = e < A.E ? max(0, w8_offset(A, e + 1) - lo) : 0;
-      const int tiles = (n + G_M - 1) / G_M;
+      const int tiles = (n + ROWS - 1) / ROWS;
       int incl = tiles;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -58,7 +91,7 @@ __global__ void __launch_bounds__(256) w8a8_generic_kernel(const W8Args A) {
       if (hit != 0) {
         const int src = __ffs(hit) - 1;
         group = e0 + src;
-        first = __shfl_sync(0xffffffffu, lo + at * G_M, src);
+        first = __shfl_sync(0xffffffffu, lo + at * ROWS, src);
       }
       before += __shfl_sync(0xffffffffu, incl, 31);
     }
@@ -69,66 +102,97 @@ __global__ void __launch_bounds__(256) w8a8_generic_kernel(const W8Args A) {
   if (group < 0) return;                           // past the last tile
   const int end = A.offsets == nullptr ? (int)A.S : w8_offset(A, group + 1);
   const int expert = group % A.period, col0 = (int)blockIdx.y * G_N;
-  const int wrows = SWIGLU ? 2 * A.N : A.N;
-  const int8_t* w = A.w + (size_t)expert * wrows * A.K;
+  const int wrows = SIDES * A.N;
+  const int8_t* const w = A.w + (size_t)expert * wrows * A.K;
   const float* ws = A.w_scale + (size_t)expert * wrows;
-  const int tx = tid & 15, ty = tid >> 4;
-  int acc[SWIGLU ? 2 : 1][4][4] = {};
-  for (int k0 = 0; k0 < A.K; k0 += G_K) {
-    for (int i = tid; i < G_M * (G_K / 4); i += 256) {
-      const int r = i / (G_K / 4), c = i % (G_K / 4), row = row0 + r;
-      s_a[r * G_LD + c] = row < end ? load_word(A.x + w8_source(A, row) * A.K, k0 + 4 * c, A.K, A.words) : 0;
-    }
+  const int8_t* const x_last = A.x + (size_t)A.T * A.K;
+  const int8_t* const w_last = A.w + (size_t)A.period * wrows * A.K;
+  // the thread's pieces: row (i * 256 + tid) / PIECES of the tile, piece tid % PIECES of the block
+  const int piece = tid % PIECES;
+  const int8_t *x_row[XP], *w_row[WP];
 #pragma unroll
-    for (int half = 0; half < (SWIGLU ? 2 : 1); ++half)
-      for (int i = tid; i < G_N * (G_K / 4); i += 256) {
-        const int n = i / (G_K / 4), c = i % (G_K / 4), col = col0 + n;
-        s_b[(half * G_N + n) * G_LD + c] =
-            col < A.N ? load_word(w + (size_t)(half * A.N + col) * A.K, k0 + 4 * c, A.K, A.words) : 0;
-      }
+  for (int i = 0; i < XP; ++i) {
+    const int row = row0 + (i * 256 + tid) / PIECES;
+    x_row[i] = row < end ? A.x + w8_source(A, row) * A.K : nullptr;
+  }
+#pragma unroll
+  for (int i = 0; i < WP; ++i) {
+    const int n = (i * 256 + tid) / PIECES, col = col0 + n % G_N;
+    w_row[i] = col < A.N ? w + (size_t)(n / G_N * A.N + col) * A.K : nullptr;
+  }
+  int4 px[XP], pw[WP];
+  auto load = [&](int k0) {
+    const int k = k0 + 16 * piece;
+#pragma unroll
+    for (int i = 0; i < XP; ++i)
+      px[i] = x_row[i] != nullptr && k < A.K ? load_piece(x_row[i], k, A.K, A.grid, A.x, x_last) : make_int4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < WP; ++i)
+      pw[i] = w_row[i] != nullptr && k < A.K ? load_piece(w_row[i], k, A.K, A.grid, A.w, w_last) : make_int4(0, 0, 0, 0);
+  };
+  const int lane = tid & 31, warp = tid >> 5, g = lane >> 2, q4 = lane & 3;
+  const int wr = ROWS == 64 ? warp / 2 * 16 : 0, wc = ROWS == 64 ? warp % 2 * 32 : warp * 8;
+  int acc[SIDES][NT][4] = {};
+  load(0);
+  for (int k0 = 0; k0 < A.K; k0 += KT) {
+#pragma unroll
+    for (int i = 0; i < XP; ++i) *reinterpret_cast<int4*>(s_x + (i * 256 + tid) / PIECES * LD + 16 * piece) = px[i];
+#pragma unroll
+    for (int i = 0; i < WP; ++i) *reinterpret_cast<int4*>(s_w + (i * 256 + tid) / PIECES * LD + 16 * piece) = pw[i];
     __syncthreads();
-#pragma unroll 4
-    for (int c = 0; c < G_K / 4; ++c) {
-      int a[4];
+    if (k0 + KT < A.K) load(k0 + KT);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = s_a[(ty + 16 * i) * G_LD + c];
+    for (int k = 0; k < KT; k += 32) {
+      auto word = [&](const int8_t* rows, int r, int at) { return *reinterpret_cast<const int*>(rows + r * LD + k + at); };
+      const int a[4] = {word(s_x, wr + g, 4 * q4), word(s_x, wr + 8 + g, 4 * q4), word(s_x, wr + g, 16 + 4 * q4),
+                        word(s_x, wr + 8 + g, 16 + 4 * q4)};
 #pragma unroll
-      for (int half = 0; half < (SWIGLU ? 2 : 1); ++half)
+      for (int side = 0; side < SIDES; ++side)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int b = s_b[(half * G_N + tx + 16 * j) * G_LD + c];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[half][i][j] = __dp4a(a[i], b, acc[half][i][j]);
+        for (int j = 0; j < NT; ++j) {
+          const int n = side * G_N + wc + 8 * j + g;
+          mma_s8(acc[side][j], a, word(s_w, n, 4 * q4), word(s_w, n, 16 + 4 * q4));
         }
     }
     __syncthreads();
   }
   OutT* out = reinterpret_cast<OutT*>(A.out);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int row = row0 + ty + 16 * i;
+  for (int half = 0; half < 2; ++half) {
+    const int row = row0 + wr + 8 * half + g;
     if (row >= end) continue;
     const float sr = A.x_scale[w8_source(A, row)];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int col = col0 + tx + 16 * j;
-      if (col >= A.N) continue;
-      float v = w8_value(acc[0][i][j], sr, ws[col]);
-      if (SWIGLU) v = w8_swiglu(v, w8_value(acc[SWIGLU ? 1 : 0][i][j], sr, ws[A.N + col]));
-      out[(size_t)row * A.N + col] = from_float<OutT>(v);
-    }
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int col = col0 + wc + 8 * j + 2 * q4 + i;
+        if (col >= A.N) continue;
+        float v = w8_value(acc[0][j][2 * half + i], sr, ws[col]);
+        if (SWIGLU) v = w8_swiglu(v, w8_value(acc[SIDES - 1][j][2 * half + i], sr, ws[A.N + col]));
+        out[(size_t)row * A.N + col] = from_float<OutT>(v);
+      }
   }
 }
 
+template <int ROWS, int KT, typename OutT>
+int launch_generic_rows(const W8Args& A, bool swiglu, cudaStream_t st) {
+  const int64_t tiles = A.S / ROWS + (A.offsets == nullptr ? 1 : (A.E < A.S ? A.E : A.S));
+  const dim3 grid((unsigned)tiles, (unsigned)((A.N + G_N - 1) / G_N));
+  if (swiglu) w8a8_generic_kernel<ROWS, KT, OutT, true><<<grid, 256, 0, st>>>(A);
+  else w8a8_generic_kernel<ROWS, KT, OutT, false><<<grid, 256, 0, st>>>(A);
+  return check_launch();
+}
+
+// Tiles of 16 rows where groups have no more, or where those of 64 would leave multiprocessors without one (K 1333, N 1499:
+// 100 rows 17.6 us, 24.5 in tiles of 64; 300 rows, 120 tiles 23.5 : 25.0; 512 rows, 192 tiles 39.5 : 28.2; K 777, N 999:
+// 3000 rows 74.3 : 41.0).
 template <typename OutT>
 int launch_generic(const W8Args& A, bool swiglu, cudaStream_t st) {
-  const int64_t tiles = A.S / G_M + (A.offsets == nullptr ? 1 : (A.E < A.S ? A.E : A.S));
-  const int64_t cols = (A.N + G_N - 1) / G_N;
+  const int64_t cols = (A.N + G_N - 1) / G_N, groups = A.E < A.S ? A.E : A.S, rows = (A.S + groups - 1) / groups;
   if (cols > 65535) return MQ_ERR_UNSUPPORTED_SHAPE;
-  const dim3 grid((unsigned)tiles, (unsigned)cols);
-  if (swiglu) w8a8_generic_kernel<OutT, true><<<grid, 256, 0, st>>>(A);
-  else w8a8_generic_kernel<OutT, false><<<grid, 256, 0, st>>>(A);
-  return check_launch();
+  if (rows > 16 && (rows + 63) / 64 * groups * cols >= device_sm_count()) return launch_generic_rows<64, 128, OutT>(A, swiglu, st);
+  return launch_generic_rows<16, 256, OutT>(A, swiglu, st);
 }
 
 int w8a8_dispatch(W8Args A, bool swiglu, int out_dtype, int32_t* d_status, cudaStream_t st) {
@@ -145,7 +209,7 @@ int w8a8_dispatch(W8Args A, bool swiglu, int out_dtype, int32_t* d_status, cudaS
     A.k_shift = (uint32_t)shift;
   }
   if (w8a8_pair_covers(A, swiglu)) return w8a8_pair(A, swiglu, out_dtype, d_status, st);
-  A.words = ((A.K | (int)(reinterpret_cast<uintptr_t>(A.x) & 3u) | (int)(reinterpret_cast<uintptr_t>(A.w) & 3u)) & 3) == 0;
+  A.grid = ((A.K | (int)(reinterpret_cast<uintptr_t>(A.x) & 15u) | (int)(reinterpret_cast<uintptr_t>(A.w) & 15u)) & 15) == 0 ? 16 : 1;
   if (out_dtype == MQ_F32) return launch_generic<float>(A, swiglu, st);
   if (out_dtype == MQ_BF16) return launch_generic<__nv_bfloat16>(A, swiglu, st);
   return launch_generic<__half>(A, swiglu, st);

@@ -15,7 +15,7 @@ struct W8Args {
   int S, T, top_k, E, period;
   int N, K;                    // N: output columns (SwiGLU: gate rows, then as many up rows)
   void* out;                   // [S, N]
-  int words;                   // rows of x and w start at multiples of four bytes
+  int grid;                    // 16: rows of x and w start at multiples of 16 bytes; else 1
   uint32_t k_mul, k_shift;     // n / top_k = umulhi(n, k_mul) >> k_shift for n < 2^31; k_mul 0: n
 };
 

@@ -96,6 +96,12 @@ def test_groups_of_256():
     lay.check(lay())
 
 
+@pytest.mark.parametrize("group,H,I", [(256, 2048, 768), (384, 1152, 768), (640, 1280, 640)])
+def test_larger_groups(group, H, I):
+    lay = Layer("w4", 9, H, I, 8, 2, group=group)
+    lay.check(lay())
+
+
 @pytest.mark.parametrize("kind,dtype", KINDS)
 def test_options(kind, dtype):
     lay = Layer(kind, 11, 256, 128, 16, 4, dtype, router_dtype=F32 if kind == "w4" else None)
