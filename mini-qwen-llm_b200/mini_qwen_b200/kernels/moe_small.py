@@ -52,7 +52,7 @@ def _call(layer: _cabi.MoELayer, x, residual, status, index) -> torch.Tensor:
         raise ValueError(f"{T} tokens of this layer (hidden {H}, inter {layer.inter}, {layer.experts} experts, top_k {layer.top_k}) "
                          "are outside what the two-launch layer covers")
     space = lib.mq_moe_small_workspace_bytes(address, T)
-    ws = torch.empty(space, dtype=torch.uint8, device=x.device)
+    ws = rows.new_empty(space, dtype=torch.uint8)
     rc = _cabi.on_device(index, lib.mq_moe_small, address, rows.data_ptr(), _cabi.ptr(residual), T, ws.data_ptr(), space,
                          out.data_ptr(), _cabi.ptr(status), _cabi.stream_ptr(index))
     if rc:

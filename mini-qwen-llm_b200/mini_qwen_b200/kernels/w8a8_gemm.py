@@ -31,14 +31,14 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     ``q = round(row / scale)``, halves to even.  A row of zeros has scale 0; a row that holds an infinity or a NaN has scale NaN
     and q 0, so that what is computed from it is NaN.  Rows may lie apart (a slice of wider rows is read in place)."""
     index = _cabi.one_device(x)
-    shape, device = x.shape, x.device
+    shape = x.shape
     if not shape or shape[-1] == 0:
         raise ValueError("rows to quantise are [..., K] with K >= 1")
     code = _cabi.dtype_code(x)
     K = shape[-1]
     rows = _apart(x, K)
-    q = torch.empty(shape, dtype=torch.int8, device=device)
-    scale = torch.empty(shape[:-1], dtype=torch.float32, device=device)
+    q = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
+    scale = x.new_empty(shape[:-1], dtype=torch.float32)
     T = rows.shape[0]
     rc = _cabi.on_device(index, _cabi.load().mq_quantize_rows_int8, rows.data_ptr(), code, T, K, rows.stride(0), q.data_ptr(),
                          scale.data_ptr(), _cabi.stream_ptr(index))
@@ -95,7 +95,7 @@ def w8a8_gemm(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, x_sc
         qweight, scales = qweight.contiguous(), scales.contiguous()
     M = x.shape[0]
     lib, stream = _cabi.load(), _cabi.stream_ptr(index)
-    out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    out = x.new_empty((M, N), dtype=out_dtype)
     word = None if status is None else status.data_ptr()
     if code is None:
         rc = _cabi.on_device(index, lib.mq_w8a8_linear, x.data_ptr(), x_scale.data_ptr(), qweight.data_ptr(), scales.data_ptr(),
@@ -105,7 +105,7 @@ def w8a8_gemm(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, x_sc
         space, ws = 0, None
         if M > 16 or M * K > 16384 or K % 16 or x.data_ptr() % 16 or qweight.data_ptr() % 16 or x.stride(0) % 8:
             space = lib.mq_w8a8_workspace_bytes(M, K, 0)
-            ws = torch.empty(space, dtype=torch.uint8, device=x.device)
+            ws = x.new_empty(space, dtype=torch.uint8)
         rc = _cabi.on_device(index, lib.mq_w8a8_linear_x, x.data_ptr(), code, x.stride(0), qweight.data_ptr(), scales.data_ptr(),
                              M, N, K, out_code, None if ws is None else ws.data_ptr(), space, out.data_ptr(), word,
                              _launches_at, stream)
@@ -149,7 +149,7 @@ def _grouped(what, x, perm, top_k, qweight, scales, expert_offsets, x_scale, zer
         raise ValueError("perm lists rows of an empty x")
     zero = out is None and zero_init
     if out is None:
-        out = torch.empty((S, N), dtype=out_dtype, device=x.device)
+        out = x.new_empty((S, N), dtype=out_dtype)
     if not (qweight.is_contiguous() and scales.is_contiguous() and expert_offsets.is_contiguous()):
         qweight, scales, expert_offsets = qweight.contiguous(), scales.contiguous(), expert_offsets.contiguous()
     wide = expert_offsets.dtype == torch.int64
@@ -158,7 +158,7 @@ def _grouped(what, x, perm, top_k, qweight, scales, expert_offsets, x_scale, zer
         launched = 1 if S else 0
         off = expert_offsets
         if S and (zero or wide):
-            narrow = torch.empty(groups + 1, dtype=torch.int32, device=x.device) if wide else None
+            narrow = x.new_empty(groups + 1, dtype=torch.int32) if wide else None
             rc = _cabi.on_device(index, lib.mq_grouped_prepare, off.data_ptr(), int(wide), S, groups, N, out_code,
                                  out.data_ptr() if zero else None, _cabi.ptr(narrow), None, stream)
             _cabi.check(rc, "mq_grouped_prepare")
@@ -172,7 +172,7 @@ def _grouped(what, x, perm, top_k, qweight, scales, expert_offsets, x_scale, zer
                                  scales.data_ptr(), *args)
     else:
         space = lib.mq_w8a8_workspace_bytes(T, K, groups)
-        ws = torch.empty(space, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(space, dtype=torch.uint8)
         rc = _cabi.on_device(index, lib.mq_w8a8_grouped_x, x.data_ptr(), code, x.stride(0), _cabi.ptr(perm), T, top_k,
                              qweight.data_ptr(), scales.data_ptr(), expert_offsets.data_ptr(), int(wide), S, groups, E, N, K,
                              int(swiglu), int(zero), out_code, ws.data_ptr(), space, out.data_ptr(), _cabi.ptr(status),
