@@ -27,8 +27,8 @@
 // a unit ahead; quotients of the scales kept from the barrier on (four divisions a lane in each unit: 22 us); scales that
 // come from afar asked for by the copying warps.  Copies alone: 7.0 to 7.5 TB/s.
 // Measured, hidden 2048, inter 768, 128 experts, top-8, weights out of L2, both launches: bf16 experts, 1 token 24 us, 8
-// tokens 83 us, 16 tokens 128 us (765 MB: 6.0 TB/s); int8, 1 token 23 us, 16 tokens 87 us; fp16, 16 tokens 145 us; int4
-// (unpacked in registers: bound by instructions), 1 token 28 us, 13 tokens 112 us.
+// tokens 83 us, 16 tokens 128 us (765 MB: 6.0 TB/s); int8, 1 token 23 us, 16 tokens 87 us; fp16, 16 tokens 136 us; int4
+// (unpacked in registers: bound by instructions), 1 token 27 us, 8 tokens 76 us, 13 tokens 112 us.
 // Every wait is bounded; when one runs out, MQ_DEV_WAIT_EXPIRED is set and the output is invalid.
 #include "int8.cuh"
 #include "tc5.cuh"
@@ -49,10 +49,11 @@ enum Format { F_BF16, F_F16, F_INT8, F_INT4 };
 
 // Who does what, by warps: [0, WARPS) multiply, the first FINISH of [WARPS, MEET) finish, the last COPY copy.  For the down
 // projection the warps of [WARPS, MEET) are a second team that takes the stages of the ring in turn with the first: for 16
-// tokens on bf16 experts 42 us instead of 52 (its work on a stage, one thing after the other, takes longer than the stage's
-// copies).  fp16 and int4 experts need more than the 96 registers of a thread that this leaves, and have one team.
-template <int F> struct Roles {
-  static constexpr int TEAMS = F == F_BF16 || F == F_INT8 ? 2 : 1, ALL = TEAMS * WARPS, MEET = TEAMS == 2 ? ALL : WARPS + FINISH;
+// tokens on bf16 experts 42 us instead of 52, fp16 51 for 62, int4 and 8 tokens 29 for 31 (its work on a stage, one thing after
+// the other, takes longer than the stage's copies).  int4 experts of more than eight tokens need more than the 96 registers of
+// a thread that this leaves.  (Both teams at gate and up as well, each finishing its tiles itself: bf16 78 us, 73 so.)
+template <int F, int OCT> struct Roles {
+  static constexpr int TEAMS = F == F_INT4 && OCT == 2 ? 1 : 2, ALL = TEAMS * WARPS, MEET = TEAMS == 2 ? ALL : WARPS + FINISH;
   static constexpr int THREADS = TEAMS == 2 ? (MEET + COPY) * 32 : MAX_T * 32;             // at least a warp for each token
   static_assert(WARPS + FINISH <= MEET && MEET + COPY <= THREADS / 32 && MAX_T <= THREADS / 32, "a warp for each role");
 };
@@ -362,12 +363,12 @@ __device__ __forceinline__ void add4(int (&s)[4], int4 v) { s[0] += v.x; s[1] +=
 struct SmallMaps { CUtensorMap gate, up, down; };  // dense and int8: gate and up rows in one
 
 template <int F, int OCT, typename OutT>
-__global__ void __launch_bounds__(Roles<F>::THREADS, 1) moe_small_layer(const SmallArgs A, const __grid_constant__ SmallMaps maps) {
+__global__ void __launch_bounds__(Roles<F, OCT>::THREADS, 1) moe_small_layer(const SmallArgs A, const __grid_constant__ SmallMaps maps) {
   using namespace tc5;
   using Acc = typename std::conditional<F == F_INT8, int, float>::type;
   constexpr int SIZE = Fmt<F>::SIZE, UNIT_K = Fmt<F>::UNIT_K, HALF_K = Fmt<F>::HALF_K, MT = Fmt<F>::MT;
   constexpr bool W4 = F == F_INT4;
-  constexpr int TEAMS = Roles<F>::TEAMS, ALL = Roles<F>::ALL, MEET = Roles<F>::MEET, THREADS = Roles<F>::THREADS;
+  constexpr int TEAMS = Roles<F, OCT>::TEAMS, ALL = Roles<F, OCT>::ALL, MEET = Roles<F, OCT>::MEET, THREADS = Roles<F, OCT>::THREADS;
   constexpr int STAGES = ring_stages(F, OCT);
   static_assert(STAGES % TEAMS == 0, "a place in the ring belongs to one team");
   extern __shared__ uint8_t small_smem_raw[];
@@ -927,20 +928,30 @@ __global__ void __launch_bounds__(Roles<F>::THREADS, 1) moe_small_layer(const Sm
       if constexpr (F == F_INT8) {
         mma_s8(c, r4.x, r84.x, r4.y, r84.y, b.x, b.y);
         mma_s8(c, r4.z, r84.z, r4.w, r84.w, b.z, b.w);
-      } else if constexpr (F == F_F16) {           // fp16 fits into tf32
-        const uint32_t r[4] = {r4.x, r4.y, r4.z, r4.w}, r8[4] = {r84.x, r84.y, r84.z, r84.w};
-        const uint4 b1 = h[i][HV - 1];
-        const uint32_t v[8] = {b.x, b.y, b.z, b.w, b1.x, b1.y, b1.z, b1.w};
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r[p]));
-          const float2 a8 = __half22float2(*reinterpret_cast<const __half2*>(&r8[p]));
-          mma_tf32(c, __float_as_uint(a.x), __float_as_uint(a8.x), __float_as_uint(a.y), __float_as_uint(a8.y), v[2 * p], v[2 * p + 1]);
-        }
       } else {
         mma_bf16(c, r4.x, r84.x, r4.y, r84.y, b.x, b.y);
         mma_bf16(c, r4.z, r84.z, r4.w, r84.w, b.z, b.w);
       }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = acc[0][i] + acc[1][i];
+  };
+  // fp16 fits into tf32.  Its h takes twice the registers, so the weights are loaded as they are needed.
+  auto multiply_f16 = [&](Acc (&sum)[4], const uint8_t* unit) {
+    float acc[2][4] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 r4 = piece(unit + (i >> 1) * (UNIT / 2), g, i & 1), r84 = piece(unit + (i >> 1) * (UNIT / 2), 8 + g, i & 1);
+      const uint32_t r[4] = {r4.x, r4.y, r4.z, r4.w}, r8[4] = {r84.x, r84.y, r84.z, r84.w};
+      const uint4 b = h[i][0], b1 = h[i][HV - 1];
+      const uint32_t v[8] = {b.x, b.y, b.z, b.w, b1.x, b1.y, b1.z, b1.w};
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&r[p]));
+        const float2 a8 = __half22float2(*reinterpret_cast<const __half2*>(&r8[p]));
+        mma_tf32(acc[i & 1], __float_as_uint(a.x), __float_as_uint(a8.x), __float_as_uint(a.y), __float_as_uint(a8.y), v[2 * p], v[2 * p + 1]);
+      }
+      asm volatile("" ::: "memory");
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum[i] = acc[0][i] + acc[1][i];
@@ -1012,8 +1023,8 @@ __global__ void __launch_bounds__(Roles<F>::THREADS, 1) moe_small_layer(const Sm
       const int chunks = live ? (tab.count(cur.place) + CHUNK - 1) / CHUNK : 0;
       if (ok) ok = mbar_wait_warp(full(stage), phase, abort_flag, A.d_status);
       const uint8_t* unit = small_smem + stage * STAGE + seat * UNIT;
-      uint4 w[W4 ? 1 : 8];
-      if constexpr (!W4) {
+      uint4 w[W4 || F == F_F16 ? 1 : 8];
+      if constexpr (!W4 && F != F_F16) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           w[2 * i] = piece(unit + (i >> 1) * (UNIT / 2), g, i & 1);
@@ -1028,6 +1039,7 @@ __global__ void __launch_bounds__(Roles<F>::THREADS, 1) moe_small_layer(const Sm
         Acc acc[4];
         if (live) {
           if constexpr (W4) multiply_int4(acc, unit, shift);
+          else if constexpr (F == F_F16) multiply_f16(acc, unit);
           else multiply_dense(acc, w);
         }
         const float of_row[2] = {row_scale[0], row_scale[1]}, of_col[2] = {col_scale[0], col_scale[1]};
@@ -1173,7 +1185,7 @@ int launch_layer(const SmallArgs& A, cudaStream_t st) {
     SmallMaps maps = {};
     if (!small_maps<F>(args, sms, maps)) return MQ_ERR_DRIVER_ENTRY;
     void* argv[] = {&args, &maps};
-    e = cudaLaunchCooperativeKernel((const void*)moe_small_layer<F, OCT, OutT>, dim3(sms), dim3(Roles<F>::THREADS), argv, smem, st);
+    e = cudaLaunchCooperativeKernel((const void*)moe_small_layer<F, OCT, OutT>, dim3(sms), dim3(Roles<F, OCT>::THREADS), argv, smem, st);
   }
   if (e != cudaSuccess) {
     cudaGetLastError();
