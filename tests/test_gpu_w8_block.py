@@ -146,3 +146,33 @@ def test_the_two_launch_layer_is_the_blocks_choice_to_make(kind):
     blk.small_layer = False
     assert torch.equal(blk(flat[1:].view(11, 256)), chain)
     blk.check_status()
+
+
+def test_layers_in_a_row():
+    """Prefill and decode steps through three W8A8 layers, eager and as one graph: a row's result does not depend on how it is
+    replayed, and follows the dense layers as closely as three quantised layers can."""
+    layers = []
+    for seed in range(3):
+        _, _, dense, q13, q2, g = make(BF16, seed=seed)
+        cfg, router = dense.config if hasattr(dense, "config") else make(BF16, seed=seed)[0], dense.gate.weight.data
+        norm = RMSNorm(256).to(DEV).to(BF16)
+        norm.weight.data.uniform_(0.8, 1.2)
+        layers.append((Qwen3MoEBlock.from_stacked_w8(cfg, router, q13, q2), dense, norm))
+
+    def run(h, which):
+        for layer in layers:
+            h = layer[which].half_layer(h, layer[2])
+        return h
+
+    for T in (33, 2, 1, 16, 17):
+        h = rows(g, T, 256, BF16)
+        out, ref = run(h, 0), run(h, 1)
+        # 2 % of a layer's addition to the residual, three times (see test_quantised_block_stays_close_to_the_dense_one)
+        assert float((out - ref).float().norm() / (ref - h).float().norm()) < 0.1
+        cap = CapturedForward(lambda x: run(x, 0), h)
+        for _ in range(2):
+            h2 = rows(g, T, 256, BF16)
+            cap.x.copy_(h2)
+            assert torch.equal(cap.replay(), run(h2, 0))
+    for layer in layers:
+        layer[0].check_status()
