@@ -376,7 +376,7 @@ int mq_w4a16_tc_swiglu(const void* xp, const float* xs,
  *   w_gate_up [weight_period, 2*I, H] (gate rows first), w_scale [weight_period, 2*I].  perm != NULL: row r of the sorted
  *   order is row perm[r] / top_k of x [T,H], gathered inside the kernel (S entries); NULL: x holds the S sorted rows, T = S.
  * Limits: Kd <= 131071 (the sums are exact in 32 bits), rows and groups < 2^30, N < 2^29.  Kd and N multiples of 16 with
- * 16-byte aligned tensors and at most 1024 groups run on the tensor cores, everything else on dot products of four bytes.
+ * 16-byte aligned tensors and at most 1024 groups run on CTA pairs, everything else in small tiles (any alignment).
  * d_status (optional) receives MQ_DEV_WAIT_EXPIRED when a bounded wait ran out; part of the result is then unwritten. */
 int mq_quantize_rows_int8(const void* x, int dtype, int64_t rows, int64_t K, int64_t row_stride, int8_t* q, float* scale,
                           void* stream);

@@ -102,7 +102,10 @@ def w4a16_moe_layer_small(hidden_states: torch.Tensor, router_weight: torch.Tens
                           group_size: int = 128, bias: torch.Tensor | None = None, renormalize: bool = True,
                           residual: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`moe_layer_small` on int4 experts: ``gate``, ``up`` and ``down`` are ``(qweight [E, K/8, N], scales [E, K/g, N],
-    qzeros [E, K/g, N/8])`` stacks as in :func:`w4a16_grouped_gemm`; bf16, group sizes that are multiples of 128."""
+    qzeros [E, K/g, N/8])`` stacks as in :func:`w4a16_grouped_gemm`; bf16, group sizes that are multiples of 128.
+
+    From about six tokens on the block's chain of launches is the faster way for int4 experts (hidden 2048, inter 768, 128
+    experts, top-8: 29 against 39 us at one token, 55 : 62 at 4, 76 : 70 at 8)."""
     index = _cabi.one_device(hidden_states, router_weight, *gate, *up, *down, bias, residual, status)
     router_weight = _router(hidden_states, router_weight)
     E, H = router_weight.shape
