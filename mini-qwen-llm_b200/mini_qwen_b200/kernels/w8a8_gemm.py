@@ -6,6 +6,7 @@ Activations are given as bf16, fp16 or fp32 rows, which the call quantises itsel
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -16,6 +17,11 @@ MAX_K = 131071      # 128 * 128 * K < 2^31: the int32 sums are exact
 
 _launches = ctypes.c_int32(0)
 _launches_at = ctypes.addressof(_launches)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(rows: int, K: int, groups: int) -> int:
+    return _cabi.load().mq_w8a8_workspace_bytes(rows, K, groups)
 
 
 def _apart(x: torch.Tensor, K: int) -> torch.Tensor:
@@ -104,7 +110,7 @@ def w8a8_gemm(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, x_sc
     else:
         space, ws = 0, None
         if M > 16 or M * K > 16384 or K % 16 or x.data_ptr() % 16 or qweight.data_ptr() % 16 or x.stride(0) % 8:
-            space = lib.mq_w8a8_workspace_bytes(M, K, 0)
+            space = _workspace_bytes(M, K, 0)
             ws = x.new_empty(space, dtype=torch.uint8)
         rc = _cabi.on_device(index, lib.mq_w8a8_linear_x, x.data_ptr(), code, x.stride(0), qweight.data_ptr(), scales.data_ptr(),
                              M, N, K, out_code, None if ws is None else ws.data_ptr(), space, out.data_ptr(), word,
@@ -171,7 +177,7 @@ def _grouped(what, x, perm, top_k, qweight, scales, expert_offsets, x_scale, zer
             rc = _cabi.on_device(index, lib.mq_w8a8_grouped_gemm, x.data_ptr(), x_scale.data_ptr(), qweight.data_ptr(),
                                  scales.data_ptr(), *args)
     else:
-        space = lib.mq_w8a8_workspace_bytes(T, K, groups)
+        space = _workspace_bytes(T, K, groups)
         ws = x.new_empty(space, dtype=torch.uint8)
         rc = _cabi.on_device(index, lib.mq_w8a8_grouped_x, x.data_ptr(), code, x.stride(0), _cabi.ptr(perm), T, top_k,
                              qweight.data_ptr(), scales.data_ptr(), expert_offsets.data_ptr(), int(wide), S, groups, E, N, K,
