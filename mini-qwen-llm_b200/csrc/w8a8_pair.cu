@@ -12,6 +12,11 @@
 // K is covered in blocks of 128; what a copy reads past K, past the last row or past the last channel is zero (the tensor
 // maps' fill), so K and N need only be multiples of 16.
 // With few rows the tiles are kept narrow, so that there is one for every pair (w8_tile_rows).
+// What bounds it: with few rows an expert HBM, with many the operands' way from L2 (a pair's stage of 64 KB takes 1.2 times as
+// long as its MMAs) and the clock under the power cap.  Measured, int8 rows given, weights out of L2 (hidden 2048, inter 768,
+// 128 experts, top-8): gate/up with the gather 58 us for 32 tokens (6.2 TB/s of weights), 70 for 512 (5.8), 115 for 4096 (1.8
+// Pop/s); down 40 for 512, 76 for 4096; a linear of 4096 rows, 2048 -> 4096 32 us (2.1 Pop/s), of 500 rows, 4096 -> 2048 10.
+// (Weights asked for ahead by tensor-map prefetches to L2: 64 tokens 69 to 87 us instead of 65.)
 // Warps: 0 copies, 1 MMA (even CTA), 2-9 epilogue, 10-13 (gathering variant) row copies.  Every wait is bounded: when one
 // runs out, MQ_DEV_WAIT_EXPIRED is set, all roles leave their loops, copies in flight are waited for and TMEM is freed.
 #include "pair.cuh"
@@ -615,8 +620,11 @@ bool w8_map_gate_up(CUtensorMap* map, const void* base, int64_t experts, int64_t
 }
 
 // Rows a tile may have: the width at which the rounds of tiles take the shortest time, by a model of a tile in clocks (the
-// MMAs' 2 a row and block of 128 k, or the copies' time where that is longer, and a fixed part), from the mean group.
-int w8_tile_rows(int64_t S, int64_t E, int64_t units, int64_t KB, int64_t pairs) {
+// MMAs' 2 a row and block of 128 k, or the copies' time where that is longer, and a fixed part) and of the last epilogue, which
+// nothing hides (16 a row, 40 with SwiGLU), from the mean group.  Of 24 sizes tried with every width the slowest choice took 7 %
+// longer than the best one (2048 tokens, 16 experts, top-4, K 1024, 512 columns: 19.8 us with 256 rows, 18.5 with 128, 24.4 with
+// 512).
+int w8_tile_rows(int64_t S, int64_t E, int64_t units, int64_t KB, int64_t pairs, bool swiglu) {
   const int64_t groups = E < S ? E : S, n = (S + groups - 1) / groups;
   int best = 512;
   double best_time = 0.0;
@@ -629,7 +637,7 @@ int w8_tile_rows(int64_t S, int64_t E, int64_t units, int64_t KB, int64_t pairs)
       stage *= 2.0;
     }
     const double rounds = tiles <= (double)pairs ? 1.0 : tiles / (double)pairs + 0.5;
-    const double time = rounds * ((double)KB * stage + 1500.0);
+    const double time = rounds * ((double)KB * stage + 1500.0) + rows * (swiglu ? 40.0 : 16.0);
     if (width == 512 || time < best_time * 0.98) {
       best = width;
       best_time = time;
@@ -640,7 +648,8 @@ int w8_tile_rows(int64_t S, int64_t E, int64_t units, int64_t KB, int64_t pairs)
 
 }  // namespace
 
-// Whole 16-byte pieces of every row of the operands and the result; coordinates and tile counts are 32-bit.
+// Whole 16-byte pieces of every row of the operands and the result; coordinates and tile counts are 32-bit.  Wherever it covers
+// a call it is the faster one (512 rows, K 1488: N 1488 8.2 us here, N 1500 16.3 in the small tiles of w8a8.cu).
 bool w8a8_pair_covers(const W8Args& A, bool swiglu) {
   return A.K % 16 == 0 && A.N % 16 == 0 && aligned16(A.x) && aligned16(A.w) && aligned16(A.out) && A.E <= W_MAX_E &&
          (int64_t)A.period * A.N * 2 < ((int64_t)1 << 31) &&
@@ -655,7 +664,7 @@ int w8a8_pair(const W8Args& A, bool swiglu, int out_dtype, int32_t* d_status, cu
       !(swiglu ? w8_map_gate_up(&map_w, A.w, A.period, A.N, A.K) : w8_map(&map_w, A.w, (int64_t)A.period * A.N, A.K, WM)))
     return MQ_ERR_DRIVER_ENTRY;
   const int64_t units = (A.N + (swiglu ? 128 : 256) - 1) / (swiglu ? 128 : 256), pairs = device_sm_count() / 2;
-  const int most = w8_tile_rows(A.S, A.E, units, (A.K + WK - 1) / WK, pairs);
+  const int most = w8_tile_rows(A.S, A.E, units, (A.K + WK - 1) / WK, pairs, swiglu);
   const int64_t tiles = ((int64_t)A.S / (most < 256 ? most : 256) + (A.E < A.S ? A.E : A.S)) * units;      // at most
   const int grid = 2 * (int)(tiles < pairs ? tiles : pairs);
 #define MQ_W8_LAUNCH(SW, GA, T)                                                                                       \

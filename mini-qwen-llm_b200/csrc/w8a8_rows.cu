@@ -162,8 +162,8 @@ size_t rows_smem_bytes(int64_t M, int64_t K) { return (size_t)M * (K + 16) + (si
 }  // namespace
 
 // Every CTA quantises all the rows, so there is a size from which a launch of its own is the faster way (us, one launch | two:
-// K 2048, N 4096: 7.8 | 13.0 for one row, 9.5 | 13.3 for 4, 11.7 | 13.3 for 8, 16.0 | 13.5 for 16; K 4096, N 4096: 16.5 | 16.2
-// for 8; 16 rows with K and N 1024: 9.3 | 10.9).
+// K 2048, N 4096: 7.4 | 13.0 for one row, 9.2 | 13.1 for 4, 11.2 | 13.2 for 8, 14.8 | 13.3 for 12, 15.3 | 13.2 for 16; K 4096,
+// N 4096: 12.8 | 15.9 for 4, 15.7 | 15.7 for 8; 16 rows with K and N 1024: 8.9 | 10.7).
 bool w8a8_rows_covers(const void* x, int x_dtype, int64_t stride, const void* w, int64_t M, int64_t N, int64_t K) {
   return M <= 16 && K % 16 == 0 && M * K <= 16384 && N < ((int64_t)1 << 30) && aligned16(x) && aligned16(w) &&
          (M == 1 || stride * (int64_t)dtype_size(x_dtype) % 16 == 0);
