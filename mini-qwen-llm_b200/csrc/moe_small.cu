@@ -6,9 +6,12 @@
 //   h[t, k] = silu(x[t] . gate[e]) * (x[t] . up[e])
 //   out[t] = round(sum_k weight[t, k] * (h[t, k] . down[e]) + residual[t])
 //
-// Everything between the inputs and the one rounding at the end is held in fp32 or better: the tensor cores' fp32 sums, and
-// h as the sum of two bf16 numbers (16 bits of precision; fp16 experts: two tf32 numbers).  W8A8: x and h are quantised per
-// token (int8.cuh), the sums are int32.
+// Everything between the inputs and the one rounding at the end is held in fp32: the tensor cores' fp32 sums, and h as the sum
+// of three bf16 numbers of eight bits each, which is the fp32 number itself.  (With two of them up to 2^-17 of h was lost, and a
+// few in a thousand bf16 results came out a step off; the third costs 0.5 us at one token, 2 us at 16, 6 with int4 experts.)
+// fp16 experts: two tf32 numbers, 2^-20 at most, and nothing is left to gain: the results of two numbers rounded to nearest,
+// 2^-22, miss their step as often (1 in 400; with fp32 throughout 1 in 500).  W8A8: x and h are quantised per token (int8.cuh),
+// the sums are int32.
 //
 // What bounds it is reading the weights of the experts that are hit; a chain of four to eight dependent launches spends more
 // than that on latencies.  So:
@@ -26,9 +29,9 @@
 // (with 2 KB and twice the warps the down projection took 66 us for 16 tokens, now 42); x, h, scales and addresses looked up
 // a unit ahead; quotients of the scales kept from the barrier on (four divisions a lane in each unit: 22 us); scales that
 // come from afar asked for by the copying warps.  Copies alone: 7.0 to 7.5 TB/s.
-// Measured, hidden 2048, inter 768, 128 experts, top-8, weights out of L2, both launches: bf16 experts, 1 token 24 us, 8
-// tokens 83 us, 16 tokens 128 us (765 MB: 6.0 TB/s); int8, 1 token 23 us, 16 tokens 87 us; fp16, 16 tokens 136 us; int4
-// (unpacked in registers: bound by instructions), 1 token 27 us, 8 tokens 76 us, 13 tokens 112 us.
+// Measured, hidden 2048, inter 768, 128 experts, top-8, weights out of L2, both launches in a graph: bf16 experts, 1 token 26 us,
+// 8 tokens 86 us, 16 tokens 130 us (765 MB: 5.9 TB/s); int8, 1 token 23 us, 16 tokens 89 us; fp16, 16 tokens 136 us; int4
+// (unpacked in registers: bound by instructions), 1 token 23 us, 8 tokens 77 us, 13 tokens 110 us.
 // Every wait is bounded; when one runs out, MQ_DEV_WAIT_EXPIRED is set and the output is invalid.
 #include "int8.cuh"
 #include "tc5.cuh"
@@ -77,7 +80,7 @@ struct SmallArgs {
   int8_t* xq;                                      // [T, H]
   int8_t* hq;                                      // [T * K, I]
   float *xs, *hs;                                  // scales: [T], [T * K]
-  void* h;                                         // [T * K, 2, I] high and low parts, bf16 (fp16 experts: tf32); int8: fp32 [T * K, I]
+  void* h;                                         // [T * K, 3, I] parts of h, bf16; fp16 experts: [T * K, 2, I], tf32; int8: fp32 [T * K, I]
   int32_t* d_status;
 };
 
@@ -788,11 +791,14 @@ __global__ void __launch_bounds__(Roles<F, OCT>::THREADS, 1) moe_small_layer(con
               }
               const float p = expf(-fabsf(gv));
               v = __fdividef(gv < 0.0f ? p * gv : gv, 1.0f + p) * uv;
-              if (F == F_BF16 || W4) {
-                __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(A.h) + row * 2 * I + col0 + col;
-                const __nv_bfloat16 high = __float2bfloat16_rn(v);
-                h[0] = high;
-                h[I] = __float2bfloat16_rn(__hisinf(high) ? 0.0f : v - __bfloat162float(high));
+              if (F == F_BF16 || W4) {             // a bf16 number is the upper 16 bits of an fp32 one; the differences are exact
+                uint16_t* h = reinterpret_cast<uint16_t*>(A.h) + row * 3 * I + col0 + col;
+                const uint32_t high = __float_as_uint(v) & 0xffff0000u;
+                const float rest = isinf(v) ? 0.0f : v - __uint_as_float(high);
+                const uint32_t middle = __float_as_uint(rest) & 0xffff0000u;
+                h[0] = (uint16_t)(high >> 16);
+                h[I] = (uint16_t)(middle >> 16);
+                h[2 * I] = (uint16_t)(__float_as_uint(rest - __uint_as_float(middle)) >> 16);
               } else if (F == F_F16) {             // a tf32 number is the upper 19 bits of an fp32 one
                 float* h = reinterpret_cast<float*>(A.h) + row * 2 * I + col0 + col;
                 const float high = __uint_as_float(__float_as_uint(v) & 0xffffe000u);
@@ -849,23 +855,25 @@ __global__ void __launch_bounds__(Roles<F, OCT>::THREADS, 1) moe_small_layer(con
   // A warp's sums of a tile, [tokens, 16 columns], are its own piece of shared memory, to which a unit's columns are added
   // with their tokens' weights.  A token that did not choose the expert takes nothing from it, whatever its weights hold.
   float* mine = reinterpret_cast<float*>(part) + warp * (128 * OCT);
-  // The columns of a product are four tokens' high parts of h and their low parts (int8: eight tokens).
-  constexpr int CHUNK = F == F_INT8 ? 8 : 4;       // tokens of a product
+  // The eight columns of a product are the parts of h of some tokens, one part after the other: three of two tokens, and two
+  // columns without (fp16: two of four tokens; int8: eight tokens).
+  constexpr int PARTS = F == F_INT8 ? 1 : F == F_F16 ? 2 : 3;
+  constexpr int CHUNK = F == F_INT8 ? 8 : F == F_F16 ? 4 : 2;              // tokens of a product
   constexpr int HS = W4 ? 8 : 4, HH = HS / 2, HV = F == F_F16 ? 2 : 1;     // steps of a unit, of a half; 16-byte pieces of a step
   constexpr int H_ITEM = F == F_INT8 ? 1 : F == F_F16 ? 4 : 2;
-  const int h_lane = (W4 ? 8 : 32 / SIZE) * q4, n_lane = F == F_INT8 ? g : g & 3;
+  const int h_lane = (W4 ? 8 : 32 / SIZE) * q4, n_lane = g % CHUNK, my_part = g / CHUNK;
   auto h_offset = [](int s) { return W4 ? 32 * s : (s >> 1) * HALF_K + (s & 1) * (16 / SIZE); };
   const uint8_t* const h_rows = F == F_INT8 ? reinterpret_cast<const uint8_t*>(A.hq)
-                                            : reinterpret_cast<const uint8_t*>(A.h) + (size_t)(g >> 2) * I * H_ITEM;
+                                            : reinterpret_cast<const uint8_t*>(A.h) + (size_t)min(my_part, PARTS - 1) * I * H_ITEM;
   uint4 h[HS][HV];
   uint32_t scale[2] = {}, zero[2] = {};                                    // int4: of the halves
   float col_scale[2] = {}, row_scale[2] = {};                              // int8: of two columns, of two tokens
   // h of a unit's tokens from `chunk` on, and the scales; the loads are a unit ahead
   auto load_h = [&](int row0, int place, int u, int chunk) {
     const int count = tab.count(place), n = chunk * CHUNK + n_lane;
-    const bool live = n < count;
+    const bool live = n < count && my_part < PARTS;
     const int row = live ? row_of(tab.at(place, n)) : 0, k0 = u * UNIT_K + h_lane, left = live ? I - k0 : 0;
-    const uint8_t* src = h_rows + ((size_t)row * (F == F_INT8 ? 1 : 2) * I + k0) * H_ITEM;
+    const uint8_t* src = h_rows + ((size_t)row * PARTS * I + k0) * H_ITEM;
 #pragma unroll
     for (int s = 0; s < HS; ++s)
 #pragma unroll
@@ -908,8 +916,9 @@ __global__ void __launch_bounds__(Roles<F, OCT>::THREADS, 1) moe_small_layer(con
     float v[4], old[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[i] = (float)acc[i];
-      if (F != F_INT8) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 2);      // the low parts' product
+      v[i] = CHUNK == 2 && q4 == PARTS ? 0.0f : (float)acc[i];             // the parts' products together
+      if (CHUNK == 2) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 1);
+      if (CHUNK <= 4) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 2);
       if (t.to[i & 1] >= 0) old[i] = mine[t.to[i & 1] + (W4 ? 1 : 8) * (i >> 1)];
     }
 #pragma unroll
@@ -1030,6 +1039,7 @@ __global__ void __launch_bounds__(Roles<F, OCT>::THREADS, 1) moe_small_layer(con
           w[2 * i] = piece(unit + (i >> 1) * (UNIT / 2), g, i & 1);
           w[2 * i + 1] = piece(unit + (i >> 1) * (UNIT / 2), 8 + g, i & 1);
         }
+        release();
       }
       for (int chunk = 0; chunk < max(chunks, 1); ++chunk) {               // more than one: loaded as they are needed
         if (chunk > 0) {
@@ -1045,7 +1055,7 @@ __global__ void __launch_bounds__(Roles<F, OCT>::THREADS, 1) moe_small_layer(con
         const float of_row[2] = {row_scale[0], row_scale[1]}, of_col[2] = {col_scale[0], col_scale[1]};
         const Target t = next;
         if (chunk + 1 >= chunks) {
-          release();
+          if (W4 || F == F_F16) release();
           load_ahead();
         }
         if (live) add(acc, t, of_row, of_col);
@@ -1102,8 +1112,8 @@ size_t carve_small(const mq_moe_layer& L, int64_t T, uint8_t* base, SmallArgs& A
   A.logits = (float*)take((size_t)(T * L.experts) * 4);
   A.xs = (float*)take((size_t)T * 4);
   A.hs = (float*)take(S * 4);
-  A.h = take(S * (size_t)L.inter * (format_of(L) == F_F16 ? 8 : 4));
   const bool int8 = format_of(L) == F_INT8;
+  A.h = take(S * (size_t)L.inter * (int8 ? 4 : format_of(L) == F_F16 ? 8 : 6));
   A.xq = int8 ? (int8_t*)take((size_t)(T * L.hidden)) : nullptr;
   A.hq = int8 ? (int8_t*)take(S * (size_t)L.inter) : nullptr;
   return used;
