@@ -293,7 +293,7 @@ struct Tables {
   uint16_t* slot;      // [T * K] token * MAX_K + which of its experts it is
   uint16_t* ids;       // [T, MAX_K] the tokens' experts
   float* w;            // [T, MAX_K] and their weights
-  __host__ __device__ static size_t bytes(int T, int E, int K) {
+  __host__ __device__ static constexpr size_t bytes(int T, int E, int K) {
     const size_t hits = (size_t)(E < T * K ? E : T * K);
     return hits * 6 + (size_t)E * 6 + (size_t)T * MAX_K * 6 + (size_t)T * K * 2 + 16;
   }
@@ -1186,7 +1186,11 @@ void launch_router(const SmallArgs& A, unsigned grid, int vec, cudaStream_t st) 
 template <int F, int OCT, typename OutT>
 int launch_layer(const SmallArgs& A, cudaStream_t st) {
   const size_t smem = front_bytes(F, OCT) + Tables::bytes(A.T, A.E, A.K) + 1024;
-  cudaError_t e = cudaFuncSetAttribute(moe_small_layer<F, OCT, OutT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  // The limit is the kernel's, not the call's: one that went by the call would be lowered by a smaller one on another thread
+  // between this line and the launch.  So always the largest.
+  constexpr size_t room = front_bytes(F, OCT) + Tables::bytes(8 * OCT, MAX_E, MAX_K) + 1024;
+  static_assert(room + 1024 <= 232448, "shared memory of a CTA, and what the kernel has of its own");
+  cudaError_t e = cudaFuncSetAttribute(moe_small_layer<F, OCT, OutT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room);
   int dev = 0, sms = 0;
   if (e == cudaSuccess) e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
