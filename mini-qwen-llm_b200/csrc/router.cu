@@ -944,9 +944,11 @@ extern "C" int mq_route_small(const void* x, int x_dtype, const void* w, int w_d
     return check_launch();
   }
   const size_t smem = (size_t)E * 8 + (size_t)T * E * 4 + (size_t)T * K * 4 + (size_t)E * 4;
+  // the kernel's limit is the largest call's: a smaller call on another thread must not lower it before this one's launch
+  constexpr size_t room = (size_t)RSM_MAX_E * 8 + (size_t)RSM_MAX_T * RSM_MAX_E * 4 + (size_t)RSM_MAX_S * 4 + (size_t)RSM_MAX_E * 4;
 #define MQ_RSM_LAUNCH(EPL)                                                                                       \
   do {                                                                                                           \
-    cudaFuncSetAttribute(route_small_kernel<EPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);       \
+    cudaFuncSetAttribute(route_small_kernel<EPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room);       \
     launch_after_predecessor(route_small_kernel<EPL>, dim3((unsigned)E), dim3(RSM_THREADS), smem, st,             \
         x, x_dtype, w, w_dtype, bias, (int)T, (int)H, (int)E, (int)K, renormalize, vec_ok, logits, counter, ids32, \
         ids64, weights, perm, inv, offsets32, offsets64, reinterpret_cast<__nv_bfloat16*>(xp), xs,                \
