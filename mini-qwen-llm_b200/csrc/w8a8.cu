@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(256) w8a8_generic_kernel(const W8Args A) {
         const int col = col0 + wc + 8 * j + 2 * q4 + i;
         if (col >= A.N) continue;
         float v = w8_value(acc[0][j][2 * half + i], sr, ws[col]);
-        if (SWIGLU) v = w8_swiglu(v, w8_value(acc[SIDES - 1][j][2 * half + i], sr, ws[A.N + col]));
+        if (SWIGLU) v = w8_swiglu<OutT>(v, w8_value(acc[SIDES - 1][j][2 * half + i], sr, ws[A.N + col]));
         out[(size_t)row * A.N + col] = from_float<OutT>(v);
       }
   }

@@ -512,7 +512,7 @@ w8a8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
               for (int q = 0; q < 2; ++q) {                                // weight rows lane / 4 and lane / 4 + 8
                 const float2 x = scaled(f[i][0][4 * j + 2 * q], f[i][0][4 * j + 2 * q + 1], s01, k.ws[0][q]);
                 const float2 y = scaled(f[i][1][4 * j + 2 * q], f[i][1][4 * j + 2 * q + 1], s01, k.ws[1][q]);
-                const float a0 = SWIGLU ? w8_swiglu(x.x, y.x) : x.x, a1 = SWIGLU ? w8_swiglu(x.y, y.y) : x.y;
+                const float a0 = SWIGLU ? w8_swiglu<OutT>(x.x, y.x) : x.x, a1 = SWIGLU ? w8_swiglu<OutT>(x.y, y.y) : x.y;
                 if (sizeof(OutT) == 4) {
                   const int r = 32 * group + 64 * (i0 + i) + 8 * j + 2 * (lane & 3), col = k.col0 + 8 * q + (lane >> 2);
                   float* o = reinterpret_cast<float*>(out) + (size_t)(k.row0 + r) * N + col;
