@@ -15,7 +15,7 @@ class LinearW8A8(nn.Module):
     Buffers: ``qweight`` int8 [N, K] (the layout of ``nn.Linear.weight``), ``scales`` fp32 [N].  ``module.to(dtype)`` must not
     touch the scales, so they stay fp32 (see ``_apply``)."""
 
-    _status = None     # device status word, allocated by the first call of more than a few rows
+    _status = None     # device status word, allocated by the first call
 
     def __init__(self, in_features: int, out_features: int):
         super().__init__()
@@ -34,8 +34,7 @@ class LinearW8A8(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         rows = x if x.dim() == 2 and x.shape[1] == self.in_features else x.reshape(-1, self.in_features)
         status = None
-        M = rows.shape[0]
-        if rows.is_cuda and (M > 16 or M * self.in_features > 16384):       # these may take a kernel with bounded waits
+        if rows.is_cuda:       # which calls take a kernel with bounded waits goes by rows, sizes and alignment
             status = self._status
             if status is None or status.device != rows.device:
                 status = self._status = torch.zeros(1, dtype=torch.int32, device=rows.device)
