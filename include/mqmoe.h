@@ -37,7 +37,8 @@ typedef enum {
   MQ_ERR_WORKSPACE_TOO_SMALL = 3,
   MQ_ERR_LAUNCH_FAILED = 4,      /* cudaGetLastError() after the launch was not cudaSuccess */
   MQ_ERR_DRIVER_ENTRY = 5,       /* cuTensorMapEncodeTiled could not be resolved or failed */
-  MQ_ERR_STATIC_SCRATCH_EXCEEDED = 6 /* the request needs more scratch than the library's built-in array */
+  MQ_ERR_STATIC_SCRATCH_EXCEEDED = 6, /* the request needs more scratch than the library's built-in array */
+  MQ_ERR_NOT_RESIDENT = 7        /* a cooperative launch whose CTAs the process's share of the GPU cannot hold at a time */
 } mq_status;
 
 /* bits of the device status word */
@@ -446,7 +447,9 @@ int mq_moe_forward(const mq_moe_layer* h_layer, const void* x, const void* norm_
  *   with hidden and inter multiples of 8; W4A16 with group sizes that are multiples of 128; W8A8 with multiples of 16.
  * workspace: mq_moe_small_workspace_bytes(layer, T) bytes, 16-byte aligned, overwritten; calls that may overlap on the GPU
  *   need one each.  x and the weights are 16-byte aligned.  The second launch is cooperative: one CTA on every SM, which
- *   wait for one another; d_status (optional) receives MQ_DEV_WAIT_EXPIRED if a wait ran out, and out is then invalid. */
+ *   wait for one another; d_status (optional) receives MQ_DEV_WAIT_EXPIRED if a wait ran out, and out is then invalid.
+ *   Where a process may not use every SM the launch is refused: MQ_ERR_NOT_RESIDENT, with nothing but the workspace written;
+ *   mq_moe_forward computes the layer there. */
 int mq_moe_small_covers(const mq_moe_layer* h_layer, int64_t T);
 size_t mq_moe_small_workspace_bytes(const mq_moe_layer* h_layer, int64_t T);
 int mq_moe_small(const mq_moe_layer* h_layer, const void* x, const void* residual, int64_t T, void* workspace,

@@ -71,6 +71,7 @@ extern "C" const char* mq_status_string(int status) {
     case MQ_ERR_STATIC_SCRATCH_EXCEEDED:
       return "request needs more scratch than the 10 MiB array built into the library (use the entry point "
              "that takes a caller workspace)";
+    case MQ_ERR_NOT_RESIDENT: return "the process's share of the GPU cannot hold the launch's CTAs at a time";
     default: return "unknown status";
   }
 }

@@ -1204,7 +1204,7 @@ int launch_layer(const SmallArgs& A, cudaStream_t st) {
   if (e != cudaSuccess) {
     cudaGetLastError();
     set_last_cuda_error(e);
-    return MQ_ERR_LAUNCH_FAILED;
+    return e == cudaErrorCooperativeLaunchTooLarge ? MQ_ERR_NOT_RESIDENT : MQ_ERR_LAUNCH_FAILED;
   }
   return check_launch();
 }

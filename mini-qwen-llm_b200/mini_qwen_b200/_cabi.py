@@ -15,6 +15,7 @@ import torch
 _LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libmqmoe.so"
 
 MQ_F32, MQ_BF16, MQ_F16 = 0, 1, 2
+MQ_ERR_NOT_RESIDENT = 7
 _DTYPES = {torch.float32: MQ_F32, torch.bfloat16: MQ_BF16, torch.float16: MQ_F16}
 
 # name -> (restype, argtypes); kept in the order of include/mqmoe.h

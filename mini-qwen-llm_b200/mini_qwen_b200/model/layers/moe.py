@@ -80,6 +80,7 @@ class _NativeLayer:
         self._small: dict = {}
         # the two-launch layer reads 16 bytes of a weight at a time
         self.aligned = all((p or 0) % 16 == 0 for p in (layer.gate[0], layer.up[0], layer.down[0]))
+        self.resident = True      # until its cooperative launch has been refused
 
     def small_workspace_bytes(self, lib, T: int) -> int:
         """Workspace of the two-launch layer, 0 where it does not cover the call."""
@@ -413,8 +414,10 @@ class Qwen3MoEBlock(nn.Module):
         if T <= 16 and (nat.layer.int8_experts if small is None else small):
             lib = _cabi.load()
             space = nat.small_workspace_bytes(lib, T)
-            if space:
-                return self._forward_small(nat, lib, x, residual, norm_weight, norm_eps, T, space, out)
+            if space and nat.resident:
+                nat.resident = self._forward_small(nat, lib, x, residual, norm_weight, norm_eps, T, space, out)
+                if nat.resident:
+                    return out
         route_ws = None
         if T <= 64:
             route_ws = self._route_ws
@@ -437,7 +440,8 @@ class Qwen3MoEBlock(nn.Module):
         return out
 
     def _forward_small(self, nat, lib, x, residual, norm_weight, norm_eps: float, T: int, space: int, out):
-        """A few tokens: the layer in two launches (three with the norm)."""
+        """A few tokens: the layer in two launches (three with the norm).  False where the second, which has a CTA on every SM,
+        is refused (a process limited to some of them): the chain computes the call."""
         stream = _cabi.stream_ptr(nat.device)
         if norm_weight is not None:
             rows = torch.empty_like(x)
@@ -451,10 +455,12 @@ class Qwen3MoEBlock(nn.Module):
         rc = _cabi.on_device(nat.device, lib.mq_moe_small, nat.address, x.data_ptr(),
                              None if residual is None else residual.data_ptr(), T, ws.data_ptr(), space, out.data_ptr(),
                              status.data_ptr(), stream)
+        _cabi.count_launches((0 if norm_weight is None else 1) + (2 if rc == 0 else 1))
+        if rc == _cabi.MQ_ERR_NOT_RESIDENT:
+            return False
         if rc:
             _cabi.check(rc, "mq_moe_small")
-        _cabi.count_launches(2 if norm_weight is None else 3)
-        return out
+        return True
 
     def _forward_staged(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         """The same chain, stage by stage: expert parallelism, stage timing and the kernels chosen by hand."""
