@@ -68,8 +68,8 @@ def _aligned(*tensors):
 
 
 def _router(x, router_weight):
-    if router_weight.dim() != 2:
-        raise ValueError("router_weight must be [experts, hidden]")
+    if router_weight.dim() != 2 or 0 in router_weight.shape:
+        raise ValueError("router_weight must be [experts, hidden], neither of them 0")
     return router_weight.contiguous()
 
 
@@ -111,12 +111,16 @@ def w4a16_moe_layer_small(hidden_states: torch.Tensor, router_weight: torch.Tens
     E, H = router_weight.shape
     if hidden_states.dtype != torch.bfloat16:
         raise ValueError("activations must be bfloat16")
-    I = gate[0].shape[-1]
+    if group_size < 128 or group_size % 128:
+        raise ValueError(f"group_size must be a multiple of 128, got {group_size}")
+    if any(t.dim() != 3 for t in (*gate, *up, *down)):
+        raise ValueError("gate, up and down are stacks of experts: (qweight, scales, qzeros), three dimensions each")
+    I = gate[0].shape[2]
     for name, trio, kd, n in (("gate", gate, H, I), ("up", up, H, I), ("down", down, I, H)):
         qw, sc, qz = trio
         if (tuple(qw.shape) != (E, kd // 8, n) or tuple(sc.shape) != (E, kd // group_size, n) or kd % group_size or n % 8
                 or tuple(qz.shape) != (E, kd // group_size, n // 8) or qw.dtype != torch.int32 or qz.dtype != torch.int32
-                or sc.dtype != torch.bfloat16 or group_size % 128):
+                or sc.dtype != torch.bfloat16):
             raise ValueError(f"{name} must be int4 stacks of [{E}, {kd}, {n}] with groups of a multiple of 128")
         _aligned(qw)
         if not (sc.is_contiguous() and qz.is_contiguous()) or sc.data_ptr() % 4:
