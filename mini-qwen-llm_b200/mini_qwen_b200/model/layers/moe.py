@@ -741,11 +741,12 @@ class Qwen3MoEBlock(nn.Module):
 
     def quantize_to_w8a8(self) -> None:
         """Replace every expert Linear by an int8 ``LinearW8A8`` (a scale for each output channel) on the same device; the
-        activations are quantised as they come, token by token.  The router stays as it is."""
+        activations are quantised as they come, token by token.  The router stays as it is.  A projection that cannot be
+        quantised (a bias, weights that are not finite) raises before any is replaced."""
         if self.ep_size > 1:
             raise ValueError("W8A8 experts do not run expert-parallel")
         if not all(isinstance(getattr(ex, p), nn.Linear) for ex in self.experts for p in _PROJ):
             raise ValueError("quantize_to_w8a8 starts from nn.Linear projections")
-        for expert in self.experts:
-            for p in _PROJ:
-                setattr(expert, p, LinearW8A8.from_float(getattr(expert, p)))
+        quantised = [(expert, p, LinearW8A8.from_float(getattr(expert, p))) for expert in self.experts for p in _PROJ]
+        for expert, p, linear in quantised:
+            setattr(expert, p, linear)
