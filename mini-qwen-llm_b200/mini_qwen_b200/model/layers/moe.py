@@ -409,6 +409,8 @@ class Qwen3MoEBlock(nn.Module):
                 return None
             if not residual.is_contiguous():
                 residual = residual.contiguous()
+            if residual.data_ptr() % 16:
+                residual = residual.clone()
         out = torch.empty_like(x)
         small = self.small_layer
         if T <= 16 and (nat.layer.int8_experts if small is None else small):
@@ -472,6 +474,8 @@ class Qwen3MoEBlock(nn.Module):
         res = None
         if residual is not None:
             res = residual.reshape(-1, shape[-1]).contiguous()
+            if res.data_ptr() % 16:                  # the combine kernel reads 16 bytes at a time
+                res = res.clone()
         K, E = self.num_experts_per_tok, self.num_experts
         st = self._ready()
         if st.get("w8") and self.ep_size > 1:
