@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import threading
 
 import torch
 
@@ -15,8 +16,15 @@ from .. import _cabi
 MAX_K = 131071      # 128 * 128 * K < 2^31: the int32 sums are exact
 
 
-_launches = ctypes.c_int32(0)
-_launches_at = ctypes.addressof(_launches)
+class _Launches(threading.local):
+    """Where a call of this host thread says how many kernels it launched."""
+
+    def __init__(self):
+        self.word = ctypes.c_int32(0)
+        self.address = ctypes.addressof(self.word)
+
+
+_launches = _Launches()
 
 
 @functools.lru_cache(maxsize=4096)
@@ -114,8 +122,8 @@ def w8a8_gemm(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, x_sc
             ws = x.new_empty(space, dtype=torch.uint8)
         rc = _cabi.on_device(index, lib.mq_w8a8_linear_x, x.data_ptr(), code, x.stride(0), qweight.data_ptr(), scales.data_ptr(),
                              M, N, K, out_code, None if ws is None else ws.data_ptr(), space, out.data_ptr(), word,
-                             _launches_at, stream)
-        launched = _launches.value
+                             _launches.address, stream)
+        launched = _launches.word.value
     if rc:
         _cabi.check(rc, "mq_w8a8_linear")
     _cabi.count_launches(launched)
@@ -182,8 +190,8 @@ def _grouped(what, x, perm, top_k, qweight, scales, expert_offsets, x_scale, zer
         rc = _cabi.on_device(index, lib.mq_w8a8_grouped_x, x.data_ptr(), code, x.stride(0), _cabi.ptr(perm), T, top_k,
                              qweight.data_ptr(), scales.data_ptr(), expert_offsets.data_ptr(), int(wide), S, groups, E, N, K,
                              int(swiglu), int(zero), out_code, ws.data_ptr(), space, out.data_ptr(), _cabi.ptr(status),
-                             _launches_at, stream)
-        launched = _launches.value
+                             _launches.address, stream)
+        launched = _launches.word.value
     if rc:
         _cabi.check(rc, what)
     _cabi.count_launches(launched)
