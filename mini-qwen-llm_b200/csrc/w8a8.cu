@@ -17,6 +17,7 @@ int w8a8_pair(const W8Args& A, bool swiglu, int out_dtype, int32_t* d_status, cu
 
 // A few rows of floating-point numbers, quantised in the same launch (w8a8_rows.cu).
 bool w8a8_rows_covers(const void* x, int x_dtype, int64_t stride, const void* w, int64_t M, int64_t N, int64_t K);
+bool w8a8_rows_pays(int64_t M, int64_t N, int64_t K);
 int w8a8_rows(const void* x, int x_dtype, int64_t stride, const int8_t* w, const float* w_scale, int64_t M, int64_t N, int64_t K,
               int out_dtype, void* out, cudaStream_t st);
 
@@ -286,12 +287,13 @@ extern "C" int mq_w8a8_linear_x(const void* x, int x_dtype, int64_t row_stride, 
   if (!sizes_fit(M, M, 1, 1, N, Kd)) return MQ_ERR_UNSUPPORTED_SHAPE;
   if (M == 0) return MQ_OK;
   if (!x || !qweight || !w_scale || !out) return MQ_ERR_INVALID_ARGUMENT;
-  if (w8a8_rows_covers(x, x_dtype, row_stride, qweight, M, N, Kd)) {
+  const bool room = workspace != nullptr && aligned16(workspace) && workspace_bytes >= mq_w8a8_workspace_bytes(M, Kd, 0);
+  if (w8a8_rows_covers(x, x_dtype, row_stride, qweight, M, N, Kd) && (w8a8_rows_pays(M, N, Kd) || !room)) {
     if (h_launches) *h_launches = 1;
     return w8a8_rows(x, x_dtype, row_stride, qweight, w_scale, M, N, Kd, out_dtype, out, reinterpret_cast<cudaStream_t>(stream));
   }
   if (!workspace || !aligned16(workspace)) return MQ_ERR_INVALID_ARGUMENT;
-  if (workspace_bytes < mq_w8a8_workspace_bytes(M, Kd, 0)) return MQ_ERR_WORKSPACE_TOO_SMALL;
+  if (!room) return MQ_ERR_WORKSPACE_TOO_SMALL;
   const W8Space ws(workspace, M, Kd);
   const int rc = mq_quantize_rows_int8(x, x_dtype, M, Kd, row_stride, ws.q, ws.scale, stream);
   if (rc != MQ_OK) return rc;

@@ -6,11 +6,14 @@
 // order, fragments of mma.sync (m16n8k32, tokens are the 8 columns), so the weights go from memory to the tensor cores without
 // a detour, and the first pieces are on their way while the CTA quantises the rows for itself (a few KB from L2, into shared
 // memory).  The warps' int32 sums meet in shared memory.
-// One row, K 2048, N 4096: 7.8 us in a graph, where two launches take 13.0.
+// One row, K 2048, N 4096: 6.9 us in a graph, where two launches take 12.3.
 #include "int8.cuh"
 #include "w8a8.cuh"
 
 namespace mq {
+
+int device_sm_count();
+
 namespace {
 
 using namespace int8;
@@ -161,12 +164,25 @@ size_t rows_smem_bytes(int64_t M, int64_t K) { return (size_t)M * (K + 16) + (si
 
 }  // namespace
 
-// Every CTA quantises all the rows, so there is a size from which a launch of its own is the faster way (us, one launch | two:
-// K 2048, N 4096: 7.4 | 13.0 for one row, 9.2 | 13.1 for 4, 11.2 | 13.2 for 8, 14.8 | 13.3 for 12, 15.3 | 13.2 for 16; K 4096,
-// N 4096: 12.8 | 15.9 for 4, 15.7 | 15.7 for 8; 16 rows with K and N 1024: 8.9 | 10.7).
+// Every CTA quantises all the rows, so there is a size of the rows from which a launch of its own is the faster way (us, one
+// launch | two: K 2048, N 4096: 6.9 | 12.3 for one row, 8.5 | 12.4 for 4, 10.5 | 12.3 for 8, 14.8 | 13.3 for 12, 15.3 | 13.2 for
+// 16; K 4096, N 4096: 12.4 | 14.9 for 4, 15.7 | 15.7 for 8; 16 rows with K and N 1024: 10.0 | 10.3).
 bool w8a8_rows_covers(const void* x, int x_dtype, int64_t stride, const void* w, int64_t M, int64_t N, int64_t K) {
   return M <= 16 && K % 16 == 0 && M * K <= 16384 && N < ((int64_t)1 << 30) && aligned16(x) && aligned16(w) &&
          (M == 1 || stride * (int64_t)dtype_size(x_dtype) % 16 == 0);
+}
+
+// The CTAs quantise the rows again in every round, two of them on an SM at a time, so N decides too.  Against the product on CTA
+// pairs (N a multiple of 16) one launch wins in a single round, and one or two short rows in two (us, one launch | two: K 2048,
+// N 8192: 10.4 | 12.7 for one row, 12.3 | 12.6 for 2, 14.4 | 12.5 for 4; 16 rows of K 64: 12.7 | 11.7; K 4096: 14.7 | 16.5 for one
+// row; N 16384: 17.4 | 15.5 and 31.3 | 15.7 for 8 rows of 2048; N 151936: 111 | 60 and 210 | 61).  Against the small tiles, which
+// walk K slowly, longer: K 4096, N 8195: 22.0 | 24.5 for 4 rows; K 16384, N 10243: 51 | 78; but K 256, N 6147: 10.3 | 8.7; K 2048,
+// N 16387: 17.5 | 16.8, 30 | 17 for 8 rows.
+bool w8a8_rows_pays(int64_t M, int64_t N, int64_t K) {
+  const int64_t rounds = ((N + 15) / 16 + 2 * device_sm_count() - 1) / (2 * device_sm_count());
+  if (rounds <= 1) return true;
+  if (N % 16 == 0) return rounds == 2 && M <= 2 && M * K <= 4096;
+  return rounds <= (M <= 2 && K >= 2048 ? 3 : M <= 4 && K >= 1024 ? 2 : 1);
 }
 
 int w8a8_rows(const void* x, int x_dtype, int64_t stride, const int8_t* w, const float* w_scale, int64_t M, int64_t N, int64_t K,

@@ -117,7 +117,8 @@ def w8a8_gemm(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor, x_sc
         launched = 1 if M else 0
     else:
         space, ws = 0, None
-        if M > 16 or M * K > 16384 or K % 16 or x.data_ptr() % 16 or qweight.data_ptr() % 16 or x.stride(0) % 8:
+        # a few rows of few enough channels are quantised and multiplied in one launch, without a workspace
+        if M > 16 or M * K > 16384 or N > 4096 or K % 16 or x.data_ptr() % 16 or qweight.data_ptr() % 16 or x.stride(0) % 8:
             space = _workspace_bytes(M, K, 0)
             ws = x.new_empty(space, dtype=torch.uint8)
         rc = _cabi.on_device(index, lib.mq_w8a8_linear_x, x.data_ptr(), code, x.stride(0), qweight.data_ptr(), scales.data_ptr(),
