@@ -648,8 +648,10 @@ int w8_tile_rows(int64_t S, int64_t E, int64_t units, int64_t KB, int64_t pairs,
 
 }  // namespace
 
-// Whole 16-byte pieces of every row of the operands and the result; coordinates and tile counts are 32-bit.  Wherever it covers
-// a call it is the faster one (512 rows, K 1488: N 1488 8.2 us here, N 1500 16.3 in the small tiles of w8a8.cu).
+// Whole 16-byte pieces of every row of the operands and the result; coordinates and tile counts are 32-bit.  Against the small
+// tiles of w8a8.cu, which it is measured against at 1 to 256 rows, K 2048 to 131056 and N 16 to 4096, it is nowhere the slower one
+// (us, here | there: K 2048, N 16 8.4 | 8.4 for any of these rows; one row of K 2048, N 4096 10.1 | 12.7, 256 rows 11.2 | 27.2; one
+// row of K 32768, N 64 38.7 | 102.8).
 bool w8a8_pair_covers(const W8Args& A, bool swiglu) {
   return A.K % 16 == 0 && A.N % 16 == 0 && aligned16(A.x) && aligned16(A.w) && aligned16(A.out) && A.E <= W_MAX_E &&
          (int64_t)A.period * A.N * 2 < ((int64_t)1 << 31) &&
