@@ -102,7 +102,8 @@ __global__ void __launch_bounds__(256) w8a8_generic_kernel(const W8Args A) {
   const int group = s_at[0], row0 = s_at[1];
   if (group < 0) return;                           // past the last tile
   const int end = A.offsets == nullptr ? (int)A.S : w8_offset(A, group + 1);
-  const int expert = group % A.period, col0 = (int)blockIdx.y * G_N;
+  const int expert = group % A.period, col0 = (int)(blockIdx.z * gridDim.y + blockIdx.y) * G_N;
+  if (col0 >= A.N) return;
   const int wrows = SIDES * A.N;
   const int8_t* const w = A.w + (size_t)expert * wrows * A.K;
   const float* ws = A.w_scale + (size_t)expert * wrows;
@@ -179,7 +180,8 @@ __global__ void __launch_bounds__(256) w8a8_generic_kernel(const W8Args A) {
 template <int ROWS, int KT, typename OutT>
 int launch_generic_rows(const W8Args& A, bool swiglu, cudaStream_t st) {
   const int64_t tiles = A.S / ROWS + (A.offsets == nullptr ? 1 : (A.E < A.S ? A.E : A.S));
-  const dim3 grid((unsigned)tiles, (unsigned)((A.N + G_N - 1) / G_N));
+  const int cols = (A.N + G_N - 1) / G_N, most = 65535;              // of a grid's second and third dimension
+  const dim3 grid((unsigned)tiles, (unsigned)(cols < most ? cols : most), (unsigned)((cols + most - 1) / most));
   if (swiglu) w8a8_generic_kernel<ROWS, KT, OutT, true><<<grid, 256, 0, st>>>(A);
   else w8a8_generic_kernel<ROWS, KT, OutT, false><<<grid, 256, 0, st>>>(A);
   return check_launch();
@@ -191,7 +193,6 @@ int launch_generic_rows(const W8Args& A, bool swiglu, cudaStream_t st) {
 template <typename OutT>
 int launch_generic(const W8Args& A, bool swiglu, cudaStream_t st) {
   const int64_t cols = (A.N + G_N - 1) / G_N, groups = A.E < A.S ? A.E : A.S, rows = (A.S + groups - 1) / groups;
-  if (cols > 65535) return MQ_ERR_UNSUPPORTED_SHAPE;
   if (rows > 16 && (rows + 63) / 64 * groups * cols >= device_sm_count()) return launch_generic_rows<64, 128, OutT>(A, swiglu, st);
   return launch_generic_rows<16, 256, OutT>(A, swiglu, st);
 }

@@ -4,7 +4,7 @@ import torch
 
 import w8a8_reference as R
 from mini_qwen_b200 import _cabi
-from mini_qwen_b200.kernels import w8a8_gemm
+from mini_qwen_b200.kernels import w8a8_gemm, w8a8_grouped_swiglu
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -34,3 +34,16 @@ def test_wide_linears(M, K, N, launches):
         rc = lib.mq_w8a8_linear_x(x.data_ptr(), 1, K, w.data_ptr(), s.data_ptr(), M, N, K, 1, ws.data_ptr() if space else None, space,
                                   alone.data_ptr(), None, None, _cabi.stream_ptr(0))
         assert rc == 0 and torch.equal(alone, out)
+
+
+@pytest.mark.parametrize("M,K,N", [(2, 3, 4194240), (2, 3, 4194241), (17, 5, 4200001)])
+def test_more_column_tiles_than_a_grid_has_in_one_dimension(M, K, N):
+    g = torch.Generator(device=DEV).manual_seed(N + M)
+    x = torch.randn(M, K, generator=g, device=DEV).bfloat16()
+    w = torch.randint(-128, 128, (N, K), generator=g, device=DEV, dtype=torch.int8)
+    s = torch.rand(N, generator=g, device=DEV) * 0.01 + 1e-4
+    q, sx = R.quantize(x)
+    R.assert_close(w8a8_gemm(x, w, s), R.product(q, sx, w, s))
+    h = w8a8_grouped_swiglu(x, w[None, :N // 2 * 2], s[None, :N // 2 * 2] * 0.05, torch.tensor([0, 1, M], dtype=torch.int32, device=DEV))
+    ref, size = R.swiglu(q, sx, w[:N // 2 * 2], s[:N // 2 * 2] * 0.05)
+    R.assert_close(h, ref, R.swiglu_extra(size))
