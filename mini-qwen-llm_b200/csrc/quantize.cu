@@ -1,6 +1,8 @@
 // Int8 rows for the W8A8 products (int8.cuh has the arithmetic).  One pass: a warp, some warps or a CTA keep their row
 // in registers between the maximum and the quotients; rows of over 32 KB, or off the 16-byte grid, are read a second time.
-// Bound by HBM: size + 1 bytes per element (32768 x 768 bf16 18.2 us, 4.2 TB/s; each further 8192 rows 3.7 us, 5.1 TB/s).
+// Bound by HBM: size + 1 bytes per element (32768 x 768 bf16 18.2 us, 4.2 TB/s; each further 8192 rows 3.7 us, 5.1 TB/s; fp32 27 us,
+// 4.7 TB/s, 32768 x 2048 of it 55 us, 6.1 TB/s).  Rows off the grid are bound by their loads, an element each (bf16, 32768 x 2047
+// 114 us, 1.8 TB/s; 8192 x 20000, over 32 KB, 249 us).
 #include <string.h>
 
 #include "int8.cuh"

@@ -146,9 +146,9 @@ class Qwen3MoEBlock(nn.Module):
         self.fuse_small_batches = True
         self.fuse_max_tokens = 64
         # up to 16 tokens: the whole layer in two launches (one rounding, at the end, instead of one after every operation).
-        # None: where the experts are W8A8 (hidden 2048, inter 768, 128 experts, top-8: 27 against 47 us at one token, 102
-        # against 115 at 16); True: wherever the call is covered (bf16 experts 31 : 47 and 148 : 158 us; int4 29 : 39 at one
-        # token, but 78 : 70 at 8); False: nowhere
+        # None: where the experts are W8A8 (hidden 2048, inter 768, 128 experts, top-8, in a graph: 23 against 38 us at one
+        # token, 95 against 97 at 16); True: wherever the call is covered (bf16 experts 27 : 42 and 138 : 146 us; int4 23 : 31 at
+        # one token, but 78 : 70 at 8); False: nowhere
         self.small_layer = None
         # expert-parallel W4A16 decode batches (at most 64 tokens over all ranks): "replicate" = every rank holds
         # all tokens and runs its own experts (two rank barriers per call), "dispatch" = the prefill path
