@@ -393,9 +393,10 @@ int mq_w8a8_grouped_swiglu(const int8_t* x, const float* x_scale, const int32_t*
 /* The same products from rows of floating-point numbers (x_dtype, row_stride elements apart), quantised by the call: what a
  * program calls that has no other use for the int8 rows.
  * mq_w8a8_linear_x: up to 16 rows of at most 16384 elements in all (Kd a multiple of 16; x, qweight and row_stride on 16-byte
- *   boundaries) need no workspace and take one launch, or, from about 4700 channels on and with a workspace, two where that is the
- *   faster way; everything else takes two.  mq_w8a8_grouped_x: mq_w8a8_grouped_gemm, or with swiglu != 0 mq_w8a8_grouped_swiglu (perm as there, else NULL);
- *   offsets of 32 or 64 bits; zero_uncovered != 0 writes zeros to the rows of out that no group covers.
+ *   boundaries) need no workspace.  They take one launch or, from about 4700 channels on and with a workspace, two where that is
+ *   the faster way; everything else takes two.
+ * mq_w8a8_grouped_x: mq_w8a8_grouped_gemm, or with swiglu != 0 mq_w8a8_grouped_swiglu (perm as there, else NULL); offsets of 32 or
+ *   64 bits; zero_uncovered != 0 writes zeros to the rows of out that no group covers.
  * workspace: mq_w8a8_workspace_bytes(rows of x, Kd, groups) bytes, 16-byte aligned, overwritten.  h_launches (optional) receives
  * the number of kernels launched. */
 size_t mq_w8a8_workspace_bytes(int64_t rows, int64_t Kd, int64_t groups);

@@ -288,6 +288,7 @@ extern "C" int mq_w8a8_linear_x(const void* x, int x_dtype, int64_t row_stride, 
   if (!sizes_fit(M, M, 1, 1, N, Kd)) return MQ_ERR_UNSUPPORTED_SHAPE;
   if (M == 0) return MQ_OK;
   if (!x || !qweight || !w_scale || !out) return MQ_ERR_INVALID_ARGUMENT;
+  // without a workspace a few rows take one launch, whatever their channels
   const bool room = workspace != nullptr && aligned16(workspace) && workspace_bytes >= mq_w8a8_workspace_bytes(M, Kd, 0);
   if (w8a8_rows_covers(x, x_dtype, row_stride, qweight, M, N, Kd) && (w8a8_rows_pays(M, N, Kd) || !room)) {
     if (h_launches) *h_launches = 1;
