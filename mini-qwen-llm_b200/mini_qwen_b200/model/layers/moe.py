@@ -109,6 +109,9 @@ class Qwen3MoEBlock(nn.Module):
     parallel: it holds only the ``num_experts / G`` experts of its rank (``experts[j]`` is global
     expert ``expert_offset + j``), routes its own tokens over all experts, and exchanges rows with
     the other ranks in one all-to-all each way (see ``mini_qwen_b200.parallel``).
+
+    Calls of one block are not to overlap on the GPU (two streams, two graphs replayed at once): up to 64 tokens are routed
+    through a workspace that the block keeps.
     """
 
     def __init__(self, config, ep_group=None, ep_mode: str = "p2p", ep_max_tokens: int | None = None):
